@@ -15,11 +15,15 @@ CSRC = os.path.join(_HERE, "csrc")
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_JIT, ERR_DEVICE_TIMEOUT, ERR_WORKSPACE = range(7)
 # dtype codes (compiler/dtype.h:14-26 of the reference)
 BOOL, INT8, INT16, INT32, INT64, UINT8, FLOAT16, FLOAT32, FLOAT64 = range(1, 10)
+BFLOAT16 = 16  # not among the reference's types
 ROUND_REF, ROUND_RNE = 0, 1
 NCHW, NHWC = 0, 1
 PATH_AUTO, PATH_SIMT, PATH_TENSOR = 0, 1, 2
 
 DTYPE_BY_NAME = {"float16": FLOAT16, "float32": FLOAT32, "float64": FLOAT64}
+# activations of Linear's epilogue
+ACTIVATIONS = {None: 0, "Relu": 1, "Gelu": 2, "GeluTanh": 3, "Swish": 4, "Sigmoid": 5, "Tanh": 6}
+MAX_TOP = 32
 EW_OPS = {"Identity": 0, "Tanh": 1, "Exp": 2, "Sigmoid": 3, "Add": 4, "Sub": 5, "Mul": 6, "Div": 7, "Constant": 8}
 
 
@@ -49,6 +53,15 @@ class QConvParams(ctypes.Structure):
         ("bias", ctypes.c_void_p), ("round_mode", ctypes.c_int32), ("clamp_hi_q", ctypes.c_int32),
         ("residual", ctypes.c_void_p), ("res_scale", ctypes.c_float), ("res_zero_point", ctypes.c_int32), ("res_relu", ctypes.c_int32),
         ("out_scale", ctypes.c_float), ("out_zero_point", ctypes.c_int32), ("fold_scales", ctypes.c_int32),
+    ]
+
+
+class LinearParams(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64), ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32), ("bias", ctypes.c_void_p), ("bias_dtype", ctypes.c_int32), ("residual_first", ctypes.c_int32),
+        ("residual", ctypes.c_void_p), ("ldr", ctypes.c_int64), ("M", ctypes.c_int64), ("O", ctypes.c_int64), ("K", ctypes.c_int64),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
     ]
 
 
@@ -123,6 +136,13 @@ SIGNATURES = {
     "chxq_conv_integer_dev": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
     "chxq_conv_dev_workspace": (_sz, [_c.POINTER(ConvGeom)]),
     "chxq_conv_integer_dev_ws": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "chxq_linear_workspace": (_sz, [_c.POINTER(LinearParams)]),
+    "chxq_linear": (_c.c_int, [_c.POINTER(LinearParams), _vp, _sz, _vp]),
+    "chxq_layernorm": (_c.c_int, [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _f32, _vp, _vp, _vp, _vp]),
+    "chxq_layernorm_grad_workspace": (_sz, [_i64, _i64]),
+    "chxq_layernorm_grad": (_c.c_int, [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "chxq_token_logprobs": (_c.c_int, [_vp, _i64, _i32, _vp, _i32, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "chxq_token_logprobs_grad": (_c.c_int, [_vp, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i64, _i64, _i32, _i64, _vp, _vp]),
 }
 
 _lib = None

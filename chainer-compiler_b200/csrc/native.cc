@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <stdarg.h>
@@ -920,27 +921,325 @@ PyObject* global_avgpool_dq(PyObject*, Args a, Py_ssize_t n) {
     OP_END
 }
 
-// x, w, b
+// ---- float operators ------------------------------------------------------------------------------------------------------
+
+int float_code(const at::Tensor& t, const char* what) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return CHXQ_FLOAT32;
+        case at::kHalf: return CHXQ_FLOAT16;
+        case at::kBFloat16: return CHXQ_BFLOAT16;
+        default: fail(CHXQ_ERR_INVALID_ARGUMENT, "%s must be float32, float16 or bfloat16, got %s", what, dtype_name(t).c_str());
+    }
+}
+
+// Device memory of a tensor: CUDA, and on the device of the call.
+void require_on(const at::Tensor& t, const at::Tensor& like, const char* what) {
+    require_cuda(t);
+    if (t.device() != like.device()) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s must be on the device of the first operand", what);
+}
+
+// Values whose bits are not what the memory holds (negated views) are written out.
+at::Tensor resolved(const at::Tensor& t) {
+    return t.is_neg() ? t.resolve_neg() : t;
+}
+
+// A tensor as rows of its last `inner` dimensions: [rows, cols] with `ld` elements from row to row.  Taken as it is where the values of a row
+// are contiguous and the rows evenly spaced, and copied where they are not or where they overlap.
+struct Rows {
+    at::Tensor t;
+    int64_t rows = 1, cols = 1, ld = 0;
+    void* data() const { return t.data_ptr(); }
+};
+
+Rows rows_of(const at::Tensor& src, int64_t inner) {
+    Rows r;
+    r.t = resolved(src);
+    const int64_t outer = r.t.dim() - inner;
+    for (int64_t d = 0; d < outer; ++d) r.rows *= r.t.size(d);
+    for (int64_t d = outer; d < r.t.dim(); ++d) r.cols *= r.t.size(d);
+    r.ld = r.cols;
+    if (r.t.is_contiguous()) return r;
+    bool ok = true;
+    int64_t want = 1;
+    for (int64_t d = r.t.dim() - 1; d >= outer && ok; --d) {
+        if (r.t.size(d) != 1 && r.t.stride(d) != want) ok = false;
+        want *= r.t.size(d);
+    }
+    int64_t pitch = -1;  // between consecutive rows; -1: no dimension of more than one row yet
+    for (int64_t d = outer - 1; d >= 0 && ok; --d) {
+        if (r.t.size(d) == 1) continue;
+        if (pitch < 0) {
+            r.ld = r.t.stride(d);
+            pitch = r.ld;
+        } else if (r.t.stride(d) != pitch) {
+            ok = false;
+        }
+        pitch *= r.t.size(d);
+    }
+    if (!ok || (r.rows > 1 && r.ld < r.cols)) {
+        r.t = r.t.contiguous();
+        r.ld = r.cols;
+    }
+    return r;
+}
+
+// The float operators run on the device of their first operand, on its current stream.
+struct OnDevice {
+    c10::cuda::CUDAGuard guard;
+    explicit OnDevice(const at::Tensor& t) : guard(t.device()) {}
+};
+
+// Frees the references of a result that is only half built when wrapping fails.
+PyObject* pack(std::vector<at::Tensor>&& ts) {
+    PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+    if (!out) throw PyErrSet{};
+    for (size_t i = 0; i < ts.size(); ++i) {
+        PyObject* o = nullptr;
+        if (ts[i].defined()) {
+            o = wrap(std::move(ts[i]));
+        } else {
+            o = Py_None;
+            Py_INCREF(o);
+        }
+        if (!o) {
+            Py_DECREF(out);
+            throw PyErrSet{};
+        }
+        PyTuple_SET_ITEM(out, (Py_ssize_t)i, o);
+    }
+    return out;
+}
+
+// x, w, b, activation code, residual, residual_first
 PyObject* linear(PyObject*, Args a, Py_ssize_t n) {
     OP_BEGIN
-    need_args("Linear", n, 3);
-    at::Tensor x = tensor(a[0], "Linear: x"), w = tensor(a[1], "Linear: w"), b;
+    need_args("Linear", n, 6);
+    const at::Tensor &x = tensor(a[0], "Linear: x"), &w = tensor(a[1], "Linear: w");
     require_cuda(x);
-    require_cuda(w);
+    require_on(w, x, "Linear: w");
+    chxq_linear_params p;
+    memset(&p, 0, sizeof(p));
+    p.dtype = float_code(x, "Linear: x");
+    if (w.scalar_type() != x.scalar_type()) fail(CHXQ_ERR_INVALID_ARGUMENT, "Linear: w must have x's dtype %s, got %s", dtype_name(x).c_str(), dtype_name(w).c_str());
+    if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1))
+        fail(CHXQ_ERR_INVALID_ARGUMENT, "Linear: x must be [..., K] and w [O, K]");
+    p.activation = (int32_t)as_long(a[3]);
+    p.residual_first = as_bool(a[5]);
+    const OnDevice on(x);
+    at::Tensor b, r0;
     if (a[2] != Py_None) {
         b = tensor(a[2], "Linear: b");
-        require_cuda(b);
-        b = b.contiguous();
+        require_on(b, x, "Linear: b");
+        if (b.numel() != w.size(0) || (b.dim() > 0 && b.size(-1) != b.numel())) fail(CHXQ_ERR_INVALID_ARGUMENT, "Linear: b must have one entry per row of w");
+        if (b.scalar_type() != x.scalar_type() && b.scalar_type() != at::kFloat)
+            fail(CHXQ_ERR_INVALID_ARGUMENT, "Linear: b must be float32 or have x's dtype %s, got %s", dtype_name(x).c_str(), dtype_name(b).c_str());
+        b = resolved(b).contiguous();
+        p.bias_dtype = float_code(b, "Linear: b");
     }
-    x = x.contiguous();
-    w = w.contiguous();
-    at::Tensor y = empty_map({x.size(0), w.size(0)}, at::kFloat, x, false);
-    call([&] {
-        return chxq_linear_f32(static_cast<const float*>(x.data_ptr()), static_cast<const float*>(w.data_ptr()),
-                               b.defined() ? static_cast<const float*>(b.data_ptr()) : nullptr, (int)x.size(0), (int)x.size(1), (int)w.size(0),
-                               static_cast<float*>(y.data_ptr()), stream());
-    });
+    std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());
+    size.back() = w.size(0);
+    Rows res;
+    if (a[4] != Py_None) {
+        r0 = tensor(a[4], "Linear: residual");
+        require_on(r0, x, "Linear: residual");
+        if (r0.sizes() != at::IntArrayRef(size) || r0.scalar_type() != x.scalar_type())
+            fail(CHXQ_ERR_INVALID_ARGUMENT, "Linear: residual must have the output's shape and x's dtype");
+        res = rows_of(r0, 1);
+        p.ldr = res.ld;
+    }
+    at::Tensor y = empty_map(size, x.scalar_type(), x, false);
+    p.O = w.size(0);
+    p.K = w.size(1);
+    if (y.numel() == 0) return wrap(std::move(y));
+    // float32 without an epilogue, the classifier of a quantized network: one k-ascending chain per output, over contiguous operands
+    const bool chain = x.scalar_type() == at::kFloat && !res.t.defined() && p.activation == CHXQ_ACT_NONE && p.K > 0;
+    const Rows xr = rows_of(chain ? resolved(x).contiguous() : x, 1), wr = rows_of(chain ? resolved(w).contiguous() : w, 1);
+    p.M = xr.rows;
+    if (chain && p.M < (1ll << 31) && p.O < (1ll << 31) && p.K < (1ll << 31)) {
+        call([&] {
+            return chxq_linear_f32(static_cast<const float*>(xr.data()), static_cast<const float*>(wr.data()),
+                                   b.defined() ? static_cast<const float*>(b.data_ptr()) : nullptr, (int)p.M, (int)p.K, (int)p.O, static_cast<float*>(y.data_ptr()),
+                                   stream());
+        });
+        return wrap(std::move(y));
+    }
+    p.x = xr.data();
+    p.ldx = xr.ld;
+    p.w = wr.data();
+    p.ldw = wr.ld;
+    p.bias = b.defined() ? b.data_ptr() : nullptr;
+    p.residual = res.t.defined() ? res.data() : nullptr;
+    p.y = y.data_ptr();
+    p.ldy = p.O;
+    OwnScratch scratch;
+    const size_t ws_bytes = chxq_linear_workspace(&p);
+    void* ws = scratch.get(ws_bytes);
+    call([&] { return chxq_linear(&p, ws, ws_bytes, stream()); });
     return wrap(std::move(y));
+    OP_END
+}
+
+// The number of dimensions from `axis` on.
+int64_t inner_dims(const at::Tensor& x, long axis, const char* op) {
+    if (axis < -x.dim() || axis >= x.dim()) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s: axis %ld is outside the %ld dimensions of x", op, axis, (long)x.dim());
+    return axis < 0 ? -axis : x.dim() - axis;
+}
+
+// scale or bias of a normalization: as many values as a row, of x's type or float32.
+at::Tensor norm_param(const at::Tensor& t, const at::Tensor& x, int64_t inner, const char* what) {
+    require_on(t, x, what);
+    if (t.sizes() != x.sizes().slice(x.dim() - inner)) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s must have the shape of the normalized dimensions", what);
+    if (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat)
+        fail(CHXQ_ERR_INVALID_ARGUMENT, "%s must be float32 or have x's dtype %s, got %s", what, dtype_name(x).c_str(), dtype_name(t).c_str());
+    return resolved(t).contiguous();
+}
+
+// x, scale, bias, axis, epsilon, stats
+PyObject* layernorm(PyObject*, Args a, Py_ssize_t n) {
+    OP_BEGIN
+    need_args("LayerNormalization", n, 6);
+    const at::Tensor& x = tensor(a[0], "LayerNormalization: x");
+    require_cuda(x);
+    const int code = float_code(x, "LayerNormalization: x");
+    const int64_t inner = inner_dims(x, as_long(a[3]), "LayerNormalization");
+    const float eps = (float)as_double(a[4]);
+    if (!(eps >= 0.f)) fail(CHXQ_ERR_INVALID_ARGUMENT, "LayerNormalization: epsilon must not be negative");
+    const bool stats = as_bool(a[5]);
+    const OnDevice on(x);
+    const at::Tensor scale = norm_param(tensor(a[1], "LayerNormalization: scale"), x, inner, "LayerNormalization: scale");
+    at::Tensor bias, mean, inv;
+    if (a[2] != Py_None) {
+        bias = norm_param(tensor(a[2], "LayerNormalization: bias"), x, inner, "LayerNormalization: bias");
+        if (bias.scalar_type() != scale.scalar_type()) fail(CHXQ_ERR_INVALID_ARGUMENT, "LayerNormalization: bias must have scale's dtype");
+    }
+    const Rows xr = rows_of(x, inner);
+    if (xr.cols < 1) fail(CHXQ_ERR_INVALID_ARGUMENT, "LayerNormalization: the normalized dimensions are empty");
+    at::Tensor y = empty_map(x.sizes(), x.scalar_type(), x, false);
+    if (stats) {
+        std::vector<int64_t> size(x.sizes().begin(), x.sizes().end());
+        for (int64_t d = x.dim() - inner; d < x.dim(); ++d) size[d] = 1;
+        mean = empty_map(size, at::kFloat, x, false);
+        inv = empty_map(size, at::kFloat, x, false);
+    }
+    if (xr.rows > 0)
+        call([&] {
+            return chxq_layernorm(xr.data(), xr.ld, code, scale.data_ptr(), bias.defined() ? bias.data_ptr() : nullptr,
+                                  scale.scalar_type() == at::kFloat ? CHXQ_FLOAT32 : code, xr.rows, xr.cols, eps, y.data_ptr(),
+                                  stats ? static_cast<float*>(mean.data_ptr()) : nullptr, stats ? static_cast<float*>(inv.data_ptr()) : nullptr, stream());
+        });
+    if (!stats) return wrap(std::move(y));
+    return pack({std::move(y), std::move(mean), std::move(inv)});
+    OP_END
+}
+
+// A statistic of a row, float32 and contiguous.
+at::Tensor row_stat(const at::Tensor& t, const at::Tensor& like, int64_t rows, const char* what) {
+    require_on(t, like, what);
+    if (t.scalar_type() != at::kFloat || t.numel() != rows) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s must be float32 with one entry per row", what);
+    return resolved(t).contiguous();
+}
+
+// dy, x, scale, mean, inv_std_dev, axis
+PyObject* layernorm_grad(PyObject*, Args a, Py_ssize_t n) {
+    OP_BEGIN
+    need_args("LayerNormalizationGrad", n, 6);
+    const at::Tensor &dy = tensor(a[0], "LayerNormalizationGrad: dy"), &x = tensor(a[1], "LayerNormalizationGrad: x");
+    require_cuda(x);
+    require_on(dy, x, "LayerNormalizationGrad: dy");
+    const int code = float_code(x, "LayerNormalizationGrad: x");
+    if (dy.scalar_type() != x.scalar_type() || dy.sizes() != x.sizes()) fail(CHXQ_ERR_INVALID_ARGUMENT, "LayerNormalizationGrad: dy must have x's shape and dtype");
+    const int64_t inner = inner_dims(x, as_long(a[5]), "LayerNormalizationGrad");
+    const OnDevice on(x);
+    const at::Tensor scale = norm_param(tensor(a[2], "LayerNormalizationGrad: scale"), x, inner, "LayerNormalizationGrad: scale");
+    const Rows xr = rows_of(x, inner), gr = rows_of(dy, inner);
+    if (xr.cols < 1) fail(CHXQ_ERR_INVALID_ARGUMENT, "LayerNormalizationGrad: the normalized dimensions are empty");
+    const at::Tensor mean = row_stat(tensor(a[3], "LayerNormalizationGrad: mean"), x, xr.rows, "LayerNormalizationGrad: mean");
+    const at::Tensor inv = row_stat(tensor(a[4], "LayerNormalizationGrad: inv_std_dev"), x, xr.rows, "LayerNormalizationGrad: inv_std_dev");
+    at::Tensor dx = empty_map(x.sizes(), x.scalar_type(), x, false);
+    at::Tensor dscale = empty_map(scale.sizes(), scale.scalar_type(), x, false), dbias = empty_map(scale.sizes(), scale.scalar_type(), x, false);
+    OwnScratch scratch;
+    const size_t ws_bytes = chxq_layernorm_grad_workspace(xr.rows, xr.cols);
+    void* ws = scratch.get(ws_bytes);
+    const bool some = xr.rows > 0;
+    call([&] {
+        return chxq_layernorm_grad(some ? gr.data() : nullptr, gr.ld, some ? xr.data() : nullptr, xr.ld, code, scale.data_ptr(),
+                                   scale.scalar_type() == at::kFloat ? CHXQ_FLOAT32 : code, some ? static_cast<const float*>(mean.data_ptr()) : nullptr,
+                                   some ? static_cast<const float*>(inv.data_ptr()) : nullptr, xr.rows, xr.cols, some ? dx.data_ptr() : nullptr, dscale.data_ptr(),
+                                   dbias.data_ptr(), ws, ws_bytes, stream());
+    });
+    return pack({std::move(dx), std::move(dscale), std::move(dbias)});
+    OP_END
+}
+
+// The tokens of rows of logits [..., V]: int32 or int64, shaped [...].
+at::Tensor token_rows(const at::Tensor& t, const at::Tensor& logits, const char* op) {
+    require_on(t, logits, "tokens");
+    if (logits.dim() < 1 || t.sizes() != logits.sizes().slice(0, logits.dim() - 1)) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s: tokens must have one entry per row of logits", op);
+    if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt) fail(CHXQ_ERR_INVALID_ARGUMENT, "%s: tokens must be int32 or int64, got %s", op, dtype_name(t).c_str());
+    return t.contiguous();
+}
+
+// logits, tokens, num_top, ignore_index
+PyObject* token_logprobs(PyObject*, Args a, Py_ssize_t n) {
+    OP_BEGIN
+    need_args("TokenLogProbs", n, 4);
+    const at::Tensor& x = tensor(a[0], "TokenLogProbs: logits");
+    require_cuda(x);
+    const int code = float_code(x, "TokenLogProbs: logits");
+    const OnDevice on(x);
+    const at::Tensor tok = token_rows(tensor(a[1], "TokenLogProbs: tokens"), x, "TokenLogProbs");
+    const long top = as_long(a[2]);
+    const bool has_ignore = a[3] != Py_None;
+    const long ignore = has_ignore ? as_long(a[3]) : 0;
+    const Rows xr = rows_of(x, 1);
+    if (xr.cols < 1) fail(CHXQ_ERR_INVALID_ARGUMENT, "TokenLogProbs: rows of logits are empty");
+    if (top < 0 || top > CHXQ_MAX_TOP || top > xr.cols)
+        fail(CHXQ_ERR_INVALID_ARGUMENT, "TokenLogProbs: num_top must be at most %d and at most the number of logits, got %ld", CHXQ_MAX_TOP, top);
+    std::vector<int64_t> size(x.sizes().begin(), x.sizes().end() - 1);
+    at::Tensor lp = empty_map(size, at::kFloat, x, false), ent = empty_map(size, at::kFloat, x, false), lse = empty_map(size, at::kFloat, x, false);
+    size.push_back(top);
+    at::Tensor top_lp = empty_map(size, at::kFloat, x, false), top_tok = empty_map(size, at::kLong, x, false);
+    if (xr.rows > 0)
+        call([&] {
+            return chxq_token_logprobs(xr.data(), xr.ld, code, tok.data_ptr(), tok.scalar_type() == at::kLong ? CHXQ_INT64 : CHXQ_INT32, xr.rows, xr.cols, (int)top,
+                                       has_ignore, ignore, static_cast<float*>(lp.data_ptr()), static_cast<float*>(ent.data_ptr()),
+                                       static_cast<float*>(lse.data_ptr()), top ? static_cast<float*>(top_lp.data_ptr()) : nullptr,
+                                       top ? static_cast<int64_t*>(top_tok.data_ptr()) : nullptr, stream());
+        });
+    return pack({std::move(lp), std::move(ent), std::move(lse), std::move(top_lp), std::move(top_tok)});
+    OP_END
+}
+
+// dlogprob, dentropy, logits, tokens, log_sum_exp, entropy, ignore_index
+PyObject* token_logprobs_grad(PyObject*, Args a, Py_ssize_t n) {
+    OP_BEGIN
+    need_args("TokenLogProbsGrad", n, 7);
+    const at::Tensor& x = tensor(a[2], "TokenLogProbsGrad: logits");
+    require_cuda(x);
+    const int code = float_code(x, "TokenLogProbsGrad: logits");
+    const OnDevice on(x);
+    const at::Tensor tok = token_rows(tensor(a[3], "TokenLogProbsGrad: tokens"), x, "TokenLogProbsGrad");
+    const Rows xr = rows_of(x, 1);
+    if (xr.cols < 1) fail(CHXQ_ERR_INVALID_ARGUMENT, "TokenLogProbsGrad: rows of logits are empty");
+    const at::Tensor lse = row_stat(tensor(a[4], "TokenLogProbsGrad: log_sum_exp"), x, xr.rows, "TokenLogProbsGrad: log_sum_exp");
+    at::Tensor dlp, dent, ent;
+    if (a[0] != Py_None) dlp = row_stat(tensor(a[0], "TokenLogProbsGrad: dlogprob"), x, xr.rows, "TokenLogProbsGrad: dlogprob");
+    if (a[1] != Py_None) {
+        dent = row_stat(tensor(a[1], "TokenLogProbsGrad: dentropy"), x, xr.rows, "TokenLogProbsGrad: dentropy");
+        if (a[5] == Py_None) fail(CHXQ_ERR_INVALID_ARGUMENT, "TokenLogProbsGrad: dentropy needs entropy");
+        ent = row_stat(tensor(a[5], "TokenLogProbsGrad: entropy"), x, xr.rows, "TokenLogProbsGrad: entropy");
+    }
+    const bool has_ignore = a[6] != Py_None;
+    const long ignore = has_ignore ? as_long(a[6]) : 0;
+    at::Tensor dx = empty_map(x.sizes(), x.scalar_type(), x, false);
+    auto floats = [](const at::Tensor& t) { return t.defined() ? static_cast<const float*>(t.data_ptr()) : nullptr; };
+    if (xr.rows > 0)
+        call([&] {
+            return chxq_token_logprobs_grad(floats(dlp), floats(dent), xr.data(), xr.ld, code, tok.data_ptr(),
+                                            tok.scalar_type() == at::kLong ? CHXQ_INT64 : CHXQ_INT32, floats(lse), floats(ent), xr.rows, xr.cols, has_ignore, ignore,
+                                            dx.data_ptr(), stream());
+        });
+    return wrap(std::move(dx));
     OP_END
 }
 
@@ -1037,7 +1336,8 @@ PyObject* setup(PyObject*, Args a, Py_ssize_t n) {
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST(quantize_linear), FAST(dequantize_linear), FAST(matmul_integer), FAST(qlinear_matmul), FAST(conv_integer), FAST(qlinear_conv),
                            FAST(qlinear_conv_packed), FAST(qlinear_conv_chain_packed), FAST(qlinear_conv_maxpool_packed), FAST(quantize_qlinear_conv_packed),
-                           FAST(conv_integer_packed), FAST(elementwise), FAST(maxpool_u8), FAST(global_avgpool_dq), FAST(linear), FAST(qadd_u8),
+                           FAST(conv_integer_packed), FAST(elementwise), FAST(maxpool_u8), FAST(global_avgpool_dq), FAST(linear), FAST(layernorm), FAST(layernorm_grad), FAST(token_logprobs),
+                           FAST(token_logprobs_grad), FAST(qadd_u8),
                            FAST(dynamic_params_u8), {"minmax", minmax, METH_O, nullptr}, FAST(transpose_map), FAST(setup),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Host bodies of the VM ops over the C ABI of libchxq.so.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};

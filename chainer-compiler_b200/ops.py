@@ -266,9 +266,53 @@ def GlobalAveragePoolDequant(x, x_scale, x_zero_point=0):
     return _native.global_avgpool_dq(x, x_scale, x_zero_point)
 
 
-def Linear(x, w, b=None):
-    """runtime/ops/connection.cc:12-15 (fp32): y = x w^T + b."""
-    return _native.linear(x, w, b)
+def _activation_code(name, op):
+    try:
+        return _lib.ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ChxqError(_lib.ERR_INVALID_ARGUMENT, "%s: unknown activation %r, must be one of %s" % (op, name, ", ".join(repr(k) for k in _lib.ACTIVATIONS)))
+
+
+def Linear(x, w, b=None, activation=None, residual=None, residual_first=False):
+    """runtime/ops/connection.cc:12-15: y = x w^T + b over the last dimension of x, with an epilogue that has no counterpart in the
+    reference: y = act(x w^T + b) + residual, or act(x w^T + b + residual) with residual_first.
+
+    x [..., K] and w [O, K] are float32, float16 or bfloat16; b [O] has their type or float32; residual has y's shape and type.
+    activation: None, "Relu", "Gelu" (erf), "GeluTanh", "Swish" (z * sigmoid(z)), "Sigmoid" or "Tanh".  Sums are held in 32 bits and rounded
+    once, after the epilogue.  Rows of x, w and residual may be cut out of wider ones (x[:, :K]); other strides are copied.
+    float32 without activation and residual keeps one k-ascending chain of fused multiply-adds per output, whatever the sizes."""
+    return _native.linear(x, w, b, _activation_code(activation, "Linear"), residual, residual_first)
+
+
+def LayerNormalization(x, scale, bias=None, axis=-1, epsilon=1e-5, stats=False):
+    """ONNX LayerNormalization over the dimensions from `axis` on: (x - mean) * inv_std_dev * scale + bias, statistics in 32 bits.
+
+    x is float32, float16 or bfloat16; scale and bias have the shape of the normalized dimensions and x's type or float32.  Returns y, or
+    (y, mean, inv_std_dev) with stats, the statistics float32 in x's shape with ones for the normalized dimensions."""
+    return _native.layernorm(x, scale, bias, axis, epsilon, stats)
+
+
+def LayerNormalizationGrad(dy, x, scale, mean, inv_std_dev, axis=-1):
+    """Gradient of LayerNormalization: (dx, dscale, dbias) from the gradient dy of y and the statistics that the forward call returned.
+    dscale and dbias have scale's type; they are sums over all rows, taken in 32 bits in an order that depends on the sizes alone."""
+    return _native.layernorm_grad(dy, x, scale, mean, inv_std_dev, axis)
+
+
+def TokenLogProbs(logits, tokens, num_top=0, ignore_index=None):
+    """Log probabilities of given tokens (or classes) under softmax(logits) with logits [..., V] and tokens [...], int32 or int64.
+
+    Returns (logprob, entropy, log_sum_exp, top_logprobs, top_tokens): float32 [...] three times, then float32 and int64 [..., num_top], the
+    most probable alternatives (num_top <= 32; equal logits by ascending index).  A token outside the row gives a logprob of NaN, one equal
+    to ignore_index 0.  Logits of -inf are forbidden values of probability zero; a row of nothing else has log probabilities of -inf and
+    entropy 0.  A row with NaN or +inf gives NaN, and NaN ranks with +inf among the alternatives."""
+    return _native.token_logprobs(logits, tokens, num_top, ignore_index)
+
+
+def TokenLogProbsGrad(dlogprob, dentropy, logits, tokens, log_sum_exp, entropy=None, ignore_index=None):
+    """Gradient of TokenLogProbs by the logits, from the gradients of logprob and entropy (float32 [...], None = 0) and the forward call's
+    log_sum_exp and entropy: dlogprob * (onehot - p) - dentropy * p * (log p + entropy), in the logits' type.  dlogprob counts as 0 where the
+    token is ignore_index."""
+    return _native.token_logprobs_grad(dlogprob, dentropy, logits, tokens, log_sum_exp, entropy, ignore_index)
 
 
 def QAddU8(a, a_scale, a_zero_point, b, b_scale, b_zero_point, y_scale, y_zero_point=0, relu=True, round_mode=ROUND_REF):

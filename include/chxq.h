@@ -45,6 +45,7 @@ extern "C" {
 #define CHXQ_FLOAT16 7
 #define CHXQ_FLOAT32 8
 #define CHXQ_FLOAT64 9
+#define CHXQ_BFLOAT16 16 /* not among the reference's types; ONNX's number */
 
 /* Rounding of QuantizeLinear and of every requantizing epilogue. */
 #define CHXQ_ROUND_REF_HALF_UP 0 /* (t + 0.5f) then truncation: runtime/ops/quantize.cc:33-34 */
@@ -371,6 +372,75 @@ int chxq_conv_integer_dev(const void* x, const void* w, const chxq_conv_geom* g,
 size_t chxq_conv_dev_workspace(const chxq_conv_geom* g);
 int chxq_conv_integer_dev_ws(const void* x, const void* w, const chxq_conv_geom* g, const void* x_zero_point, const void* w_zero_point,
                              int64_t w_zp_len, int32_t* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Float operators around the 8-bit path: the products, normalizations and losses of a network whose other layers are quantized.
+ * Element types CHXQ_FLOAT32, CHXQ_FLOAT16 and CHXQ_BFLOAT16; sums and statistics are held in 32 bits and rounded once.  Rows may be cut
+ * out of wider ones: ld* is the distance of two rows in elements (not looked at when there is one row).  Extents may be zero. */
+
+/* Activations of chxq_linear's epilogue. */
+#define CHXQ_ACT_NONE 0
+#define CHXQ_ACT_RELU 1
+#define CHXQ_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */
+#define CHXQ_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define CHXQ_ACT_SWISH 4     /* z / (1 + exp(-z)) */
+#define CHXQ_ACT_SIGMOID 5
+#define CHXQ_ACT_TANH 6
+
+/* Linear (runtime/ops/connection.cc:12-15) with an epilogue:
+ *   y[m, o] = act(sum_k x[m, k] w[o, k] + bias[o]) + residual[m, o], or, with residual_first, act(... + residual[m, o]).
+ * x [M, ldx], w [O, ldw], residual [M, ldr] and y [M, ldy] have the type `dtype`; bias [O] has it too or is fp32; bias and residual may be
+ * NULL.  y may be the residual's memory (same ldy and ldr), and none of the other operands'.
+ * chxq_linear_workspace reads the extents, pitches and the alignment of the addresses. */
+typedef struct chxq_linear_params {
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;
+    int32_t dtype;
+    int32_t activation;
+    const void* bias;
+    int32_t bias_dtype;
+    int32_t residual_first;
+    const void* residual;
+    int64_t ldr;
+    int64_t M, O, K;
+    void* y;
+    int64_t ldy;
+} chxq_linear_params;
+size_t chxq_linear_workspace(const chxq_linear_params* p);
+int chxq_linear(const chxq_linear_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* LayerNormalization of each row's D values, D >= 1: y = (x - mean) * inv_std_dev * scale + bias, inv_std_dev = 1 / sqrt(mean of squared
+ * deviations + epsilon).  scale, bias [D] of x's type or fp32, bias may be NULL; y [rows, D] of x's type, not x's memory; mean and
+ * inv_std_dev [rows] may be NULL. */
+int chxq_layernorm(const void* x, int64_t ldx, int32_t dtype, const void* scale, const void* bias, int32_t affine_dtype, int64_t rows, int64_t D,
+                   float epsilon, void* y, float* mean, float* inv_std_dev, void* stream);
+/* Its gradient.  With xh = (x - mean) inv_std_dev and g = dy scale:
+ *   dx = inv_std_dev (g - mean(g) - xh mean(g xh)),  dscale = sum over the rows of dy xh,  dbias = sum over the rows of dy.
+ * dx [rows, D] of x's type, dscale and dbias [D] of scale's type; dbias may be NULL.  The order of the sums depends on the extents alone:
+ * the same call gives the same bits. */
+size_t chxq_layernorm_grad_workspace(int64_t rows, int64_t D);
+int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype, const void* scale, int32_t affine_dtype,
+                        const float* mean, const float* inv_std_dev, int64_t rows, int64_t D, void* dx, void* dscale, void* dbias, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens.  Per row of V >= 1 logits:
+ *   log_sum_exp = log sum exp(logit),  logprob = logit[token] - log_sum_exp,  entropy = -sum p log p,
+ *   top_tokens / top_logprobs [num_top]: the largest logits, equal ones by ascending index, num_top <= min(V, CHXQ_MAX_TOP).
+ * tokens are CHXQ_INT32 or CHXQ_INT64.  A token outside the row gives logprob NaN; one equal to ignore_index (has_ignore != 0) gives 0.
+ * A logit of -infinity has probability zero; a row of nothing else has log_sum_exp and log probabilities of -infinity and entropy 0.  A row
+ * with a NaN or +infinity gives NaN (NaN ranks with +infinity). */
+#define CHXQ_MAX_TOP 32
+int chxq_token_logprobs(const void* logits, int64_t ld, int32_t dtype, const void* tokens, int32_t token_dtype, int64_t rows, int64_t V,
+                        int32_t num_top, int32_t has_ignore, int64_t ignore_index, float* logprob, float* entropy, float* log_sum_exp,
+                        float* top_logprobs, int64_t* top_tokens, void* stream);
+/* The gradient by the logits, from the gradients of logprob and entropy (either may be NULL = 0; dentropy needs entropy):
+ *   dlogits[j] = dlogprob (1[j = token] - p_j) - dentropy p_j (log p_j + entropy)
+ * dlogits [rows, V] of the logits' type; dlogprob counts as 0 in rows whose token is ignore_index and gives NaN in rows whose token lies
+ * outside. */
+int chxq_token_logprobs_grad(const float* dlogprob, const float* dentropy, const void* logits, int64_t ld, int32_t dtype, const void* tokens,
+                             int32_t token_dtype, const float* log_sum_exp, const float* entropy, int64_t rows, int64_t V, int32_t has_ignore,
+                             int64_t ignore_index, void* dlogits, void* stream);
 
 #ifdef __cplusplus
 }
