@@ -1,0 +1,112 @@
+// The float matrix product on the tensor cores: what its two kernels (linear_tile.cuh, linear_pair.cuh) share.
+#pragma once
+
+#include <cuda.h>
+
+#include "epilogue_float.cuh"
+#include "tc_kernel3.cuh"
+
+namespace chxq {
+namespace lin {
+
+using namespace tc;
+
+struct TcArgs {
+    int M, O;       // rows of x, rows of w
+    int k_blocks;   // K in blocks of 128 bytes
+    uint32_t idesc;  // instruction descriptor without its extents
+    LinearEpilogue e;
+    int vec;  // rows of y and of the residual start on 16-byte boundaries and hold whole groups of 16 bytes
+    int* status;
+    unsigned long long wait_limit_ns;
+};
+
+// Instruction descriptor of tcgen05.mma kind::f16: 32-bit accumulator, both operands K-major and of one type.
+constexpr uint32_t kF16 = 0u, kBf16 = 1u;
+inline uint32_t idesc_f16(uint32_t type) {
+    return (1u << 4) | (type << 7) | (type << 10);
+}
+__host__ __device__ constexpr uint32_t idesc_extents(int m, int n) {
+    return ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// D[tmem] (+)= A B^T over 32 bytes of K of each operand, kind::f16, issued by one thread; PAIR: over a CTA pair (M = 256).
+template <bool PAIR>
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+                "{\n\t"
+                ".reg .pred p;\n\t"
+                ".reg .b64 da, db;\n\t"
+                "mov.b64 da, {%1, %3};\n\t"
+                "mov.b64 db, {%2, %3};\n\t"
+                "setp.ne.b32 p, %5, 0;\n\t"
+                "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t"
+                "}\n" ::"r"(tmem_d),
+                "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+                : "memory");
+    else
+        asm volatile(
+                "{\n\t"
+                ".reg .pred p;\n\t"
+                ".reg .b64 da, db;\n\t"
+                "mov.b64 da, {%1, %3};\n\t"
+                "mov.b64 db, {%2, %3};\n\t"
+                "setp.ne.b32 p, %5, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+                "}\n" ::"r"(tmem_d),
+                "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+                : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src),
+                 "r"(c0), "r"(c1)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// A barrier over `threads` threads that tells each of them whether `ok` held for all.
+__device__ __forceinline__ bool bar_all(int id, int threads, bool ok) {
+    uint32_t r;
+    asm volatile(
+            "{\n\t"
+            ".reg .pred p, q;\n\t"
+            "setp.ne.u32 p, %3, 0;\n\t"
+            "bar.red.and.pred q, %1, %2, p;\n\t"
+            "selp.u32 %0, 1, 0, q;\n\t"
+            "}\n"
+            : "=r"(r)
+            : "r"(id), "r"(threads), "r"((uint32_t)ok)
+            : "memory");
+    return r != 0;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack16(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack16<__half>(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack16<__nv_bfloat16>(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+}  // namespace lin
+}  // namespace chxq

@@ -111,6 +111,23 @@ int encode_nhwc_box_map(CUtensorMap* out, const void* base, int C, int W, int H,
     if (r != CUDA_SUCCESS) return set_error(CHXQ_ERR_CUDA, "cuTensorMapEncodeTiled(NHWC box) failed with %d", (int)r);
     return CHXQ_OK;
 }
+
+int encode_rows_map(CUtensorMap* out, const void* base, int64_t row_bytes, int64_t rows, int64_t ld_bytes, int box_rows) {
+    EncodeTiledFn encode = get_encode_fn();
+    if (!encode) return set_error(CHXQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(rows == 1 ? (row_bytes + 15) / 16 * 16 : ld_bytes)};  // one row has no pitch
+    const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(CHXQ_ERR_CUDA, "cuTensorMapEncodeTiled(rows) failed with %d", (int)r);
+    return CHXQ_OK;
+}
+
+int sm_count() {
+    return num_sms();
+}
 }  // namespace tc
 
 int choose_bk(int k) {

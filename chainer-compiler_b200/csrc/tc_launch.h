@@ -109,5 +109,10 @@ long long wait_limit_ns_value();  // limit of the bounded device-side waits (chx
 // box_c bytes (a multiple of 16) x box_w pixels x box_h rows of one image; reads outside the map fill 0.
 int encode_nhwc_box_map(CUtensorMap* out, const void* base, int C, int W, int H, int N, int64_t cs, int box_c, int box_w, int box_h);
 
+// Tensor map over rows of `row_bytes` bytes, ld_bytes apart (a multiple of 16, base 16-byte aligned); a box is 128 bytes of box_rows rows, stored
+// with the 128-byte swizzle; reads outside fill 0.
+int encode_rows_map(CUtensorMap* out, const void* base, int64_t row_bytes, int64_t rows, int64_t ld_bytes, int box_rows);
+int sm_count();  // of the current device
+
 }  // namespace tc
 }  // namespace chxq
