@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace chxq {
@@ -56,6 +58,96 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
     if (dtype == CHXQ_FLOAT32) static_cast<float*>(p)[i] = v;
     else if (dtype == CHXQ_FLOAT16) static_cast<__half*>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// N consecutive values as one load or store of N * sizeof(T) bytes (2, 4 or 16): the address is a multiple of that.
+template <typename T, int N>
+struct Pack {
+    static constexpr int kBytes = N * (int)sizeof(T), kWords = kBytes >= 4 ? kBytes / 4 : 1;
+    static_assert(kBytes == 2 || kBytes == 4 || kBytes == 16, "no such access");
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kBytes == 16) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if constexpr (kBytes == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+        else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t v = w[i >> 1];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+        const uint16_t h = (uint16_t)(i & 1 ? v >> 16 : v);
+        return __half2float(*reinterpret_cast<const __half*>(&h));
+    }
+    __device__ __forceinline__ void set(const float (&f)[N]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = __float_as_uint(f[i]);
+        } else if constexpr (N == 1) {
+            const T h = from_f32<T>(f[0]);
+            w[0] = *reinterpret_cast<const uint16_t*>(&h);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[i], f[i + 1]);
+                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __half2 h = __floats2half2_rn(f[i], f[i + 1]);
+                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+        }
+    }
+};
+
+// N consecutive values of a parameter array (N from a Pack of some 2-, 4- or 16-byte access; the array starts on a 16-byte boundary where N > 1).
+template <int N>
+__device__ __forceinline__ void load_params(const FloatArray& a, int64_t i, float (&f)[N]) {
+    if (a.dtype == CHXQ_FLOAT32) {
+        const float* p = static_cast<const float*>(a.p) + i;
+        if constexpr (N >= 4) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(p + j));
+                f[j] = v.x; f[j + 1] = v.y; f[j + 2] = v.z; f[j + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) f[j] = __ldg(p + j);
+        }
+    } else if constexpr (N == 8) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p) + i));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (a.dtype == CHXQ_BFLOAT16) {
+                f[2 * j] = __uint_as_float(w[j] << 16);
+                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+                f[2 * j] = h.x;
+                f[2 * j + 1] = h.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = load_param(a, i + j);
+    }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
