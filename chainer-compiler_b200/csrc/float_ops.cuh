@@ -60,6 +60,34 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// Two 32-bit values per instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 make_x2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split_x2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // N consecutive values as one load or store of N * sizeof(T) bytes (2, 4 or 16): the address is a multiple of that.
 template <typename T, int N>
 struct Pack {
@@ -86,12 +114,41 @@ struct Pack {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) w[i] = 0u;
     }
+    __device__ __forceinline__ void put(int i, T v) {  // into a zero
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v);
+        else w[i >> 1] |= (uint32_t)*reinterpret_cast<const uint16_t*>(&v) << (i & 1 ? 16 : 0);
+    }
     __device__ __forceinline__ float get(int i) const {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
         const uint32_t v = w[i >> 1];
         if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
         const uint16_t h = (uint16_t)(i & 1 ? v >> 16 : v);
         return __half2float(*reinterpret_cast<const __half*>(&h));
+    }
+    __device__ __forceinline__ f32x2 pair(int i) const {  // values 2 i and 2 i + 1
+        if constexpr (sizeof(T) == 4) return make_x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else return make_x2(get(2 * i), get(2 * i + 1));
+    }
+    __device__ __forceinline__ void set_pair(int i, f32x2 v) {
+        const float2 f = split_x2(v);
+        if constexpr (sizeof(T) == 4) {
+            w[2 * i] = __float_as_uint(f.x);
+            w[2 * i + 1] = __float_as_uint(f.y);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __half2 h = __floats2half2_rn(f.x, f.y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    __device__ __forceinline__ T value(int i) const {  // as it is stored
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[i]);
+        } else {
+            const uint16_t h = (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]);
+            return *reinterpret_cast<const T*>(&h);
+        }
     }
     __device__ __forceinline__ void set(const float (&f)[N]) {
         if constexpr (sizeof(T) == 4) {
@@ -147,6 +204,20 @@ __device__ __forceinline__ void load_params(const FloatArray& a, int64_t i, floa
     } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) f[j] = load_param(a, i + j);
+    }
+}
+
+// The same from any place: N loads, of T or of 32 bits.
+template <typename T, int N>
+__device__ __forceinline__ void load_params_any(const FloatArray& a, int64_t i, float (&f)[N]) {
+    if (a.dtype == CHXQ_FLOAT32) {
+        const float* p = static_cast<const float*>(a.p) + i;
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = __ldg(p + j);
+    } else {
+        const T* p = static_cast<const T*>(a.p) + i;
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = to_f32(p[j]);
     }
 }
 
