@@ -142,6 +142,26 @@ struct Pack {
             w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
+    __device__ __forceinline__ float max_value() const {  // NaN if there is one; N > 1
+        if constexpr (sizeof(T) == 4) {
+            float m = __uint_as_float(w[0]);
+#pragma unroll
+            for (int i = 1; i < kWords; ++i) asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(m), "f"(__uint_as_float(w[i])));
+            return m;
+        } else {
+            uint32_t m = w[0];
+#pragma unroll
+            for (int i = 1; i < kWords; ++i) {
+                if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+                else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[i]));
+            }
+            Pack<T, 2> p;
+            p.w[0] = m;
+            float r;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(p.get(0)), "f"(p.get(1)));
+            return r;
+        }
+    }
     __device__ __forceinline__ T value(int i) const {  // as it is stored
         if constexpr (sizeof(T) == 4) {
             return __uint_as_float(w[i]);

@@ -3,27 +3,302 @@
 //   lse = log sum exp x,  lp = x[token] - lse,  H = -sum p log p = lse - sum p x
 //   dx_j = g (1[j = token] - p_j) - h p_j (log p_j + H)
 // A logit of -infinity is a forbidden value: it has probability zero and adds nothing.
+#include <algorithm>
+
 #include "float_ops.cuh"
+#include "pdl.cuh"
+#include "tc_kernel.cuh"  // cluster helpers
 
 namespace chxq {
 namespace {
 
-constexpr int kThreads = 256;
-
-struct Best {
-    float v;
-    int i;
-};
-__device__ __forceinline__ bool before(const Best& a, const Best& b) {  // a ranks before b: the larger value, then the lower index
-    return a.v > b.v || (a.v == b.v && a.i < b.i);
-}
-__device__ __forceinline__ float rank_value(float v) {  // NaN ranks with +infinity
-    return v != v ? INFINITY : v;
-}
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ int64_t load_token(const void* tokens, int dtype, int64_t r) {
     return dtype == CHXQ_INT64 ? static_cast<const int64_t*>(tokens)[r] : (int64_t)static_cast<const int32_t*>(tokens)[r];
 }
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float a) {  // good to 2^-22
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+    return r;
+}
+
+// ---- sums -----------------------------------------------------------------------------------------------------------------
+
+// A part of a row: its largest logit m, s = sum exp(x - m) and t = sum exp(x - m) (x - m).  Without a logit above -infinity: m = -infinity, s = t = 0.
+struct Part {
+    float m, s, t;
+};
+__device__ __forceinline__ void rescale(Part& a, float m) {  // to a larger maximum
+    // below -10000 the factor is zero, and its product with the difference has to be: the difference must stay finite
+    const float d = max_nan(a.m - m, -1e4f), f = a.m == -INFINITY ? 0.f : __expf(d);
+    a.t = a.m == -INFINITY ? 0.f : f * fmaf(a.s, d, a.t);
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ Part join(Part a, Part b) {
+    const float m = max_nan(a.m, b.m);
+    if (m == -INFINITY) return a;
+    rescale(a, m);
+    rescale(b, m);
+    return {m, a.s + b.s, a.t + b.t};
+}
+
+// ---- the best alternatives ------------------------------------------------------------------------------------------------
+
+// A list of 32 logits in descending order, one per lane; equal ones by ascending index; empty places are (-infinity, kNone), behind everything.
+constexpr int kNone = 0x7fffffff;
+struct Entry {
+    float v;
+    int i;
+};
+__device__ __forceinline__ bool before(float va, int ia, float vb, int ib) {
+    return va > vb || (va == vb && ia < ib);
+}
+__device__ __forceinline__ float rank_value(float v) {  // NaN ranks with +infinity
+    return v != v ? INFINITY : v;
+}
+// Puts (v, i), the same for all lanes, in its place.
+__device__ __forceinline__ void insert(Entry& e, float v, int i) {
+    const int lane = threadIdx.x & 31;
+    const int pos = __popc(__ballot_sync(0xffffffffu, before(e.v, e.i, v, i)));
+    const float uv = __shfl_up_sync(0xffffffffu, e.v, 1);
+    const int ui = __shfl_up_sync(0xffffffffu, e.i, 1);
+    if (lane > pos) e = {uv, ui};
+    if (lane == pos) e = {v, i};
+}
+// The best 32 of two lists: the larger of one and the reversed other is a bitonic sequence of them, which five steps sort.
+__device__ __forceinline__ void merge(Entry& e, Entry o) {
+    const int lane = threadIdx.x & 31;
+    o.v = __shfl_sync(0xffffffffu, o.v, 31 - lane);
+    o.i = __shfl_sync(0xffffffffu, o.i, 31 - lane);
+    if (before(o.v, o.i, e.v, e.i)) e = o;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const float v = __shfl_xor_sync(0xffffffffu, e.v, d);
+        const int i = __shfl_xor_sync(0xffffffffu, e.i, d);
+        if (before(v, i, e.v, e.i) == ((lane & d) == 0)) e = {v, i};
+    }
+}
+// The lanes' values in descending order.
+__device__ __forceinline__ float sort_lanes(float v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            const float o = __shfl_xor_sync(0xffffffffu, v, d);
+            const bool up = (lane & size) == 0, low = (lane & d) == 0;
+            v = (up == low) ? fmaxf(v, o) : fminf(v, o);
+        }
+    return v;
+}
+__device__ __forceinline__ float merge_lanes(float v, float o) {  // the best 32 of two sorted sets of lanes, sorted
+    const int lane = threadIdx.x & 31;
+    v = fmaxf(v, __shfl_sync(0xffffffffu, o, 31 - lane));
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const float q = __shfl_xor_sync(0xffffffffu, v, d);
+        v = (lane & d) == 0 ? fmaxf(v, q) : fminf(v, q);
+    }
+    return v;
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------------
+
+struct LogprobArgs {
+    const void* tokens;
+    int token_dtype, num_top, has_ignore;
+    int64_t rows, ignore;
+    float *logprob, *entropy, *lse, *top_lp;
+    int64_t* top_tok;
+};
+
+// One pass over a row: the running maximum and the two sums of a thread are rescaled when the maximum grows.  W warps take a row (one for short rows, else
+// the block's eight), or the blocks of a cluster (W = 8) a part of it each; the parts meet in shared memory, and the blocks' in the first block's
+// through distributed shared memory.  A thread has kU accesses of sixteen bytes in flight; up to 15 bytes at either end of a row are read one by one.
+// Alternatives (TOP): a warp keeps its best 32 logits, one per lane.  Few logits get as far as the insertion: after the first round of accesses the num_top-th
+// largest of the threads' maxima bounds the num_top-th best from below, and so does the list itself.
+// Bound: HBM; per logit one conversion, one maximum, four instructions on pairs, a clamp and an exponential.
+template <typename T, int W, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, int split, const LogprobArgs p) {
+    constexpr int VEC = 16 / (int)sizeof(T), kU = 4;
+    constexpr uint32_t kNegInf = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+    __shared__ Part parts[kWarps];
+    __shared__ Entry lists[TOP ? kWarps : 1][32];
+    __shared__ float maxima[TOP ? kWarps : 1][32];
+    pdl_launch_dependents();
+    pdl_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : (int64_t)blockIdx.x / split;
+    if (W == 1 && r >= p.rows) return;
+    const int rank = W == 1 ? 0 : (int)(blockIdx.x % split);
+    const T* x = logits + r * ld;
+    const int head = min(V, (int)((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / (int)sizeof(T));
+    const int pieces = (V - head) / VEC, tail = V - head - pieces * VEC;
+    const int p0 = (int)((int64_t)pieces * rank / split), p1 = (int)((int64_t)pieces * (rank + 1) / split);
+    const T* body = x + head;
+    constexpr int kLanes = W * 32;
+    const int t = W == 1 ? lane : (int)threadIdx.x;
+
+    float m = -INFINITY;
+    f32x2 s2 = 0ull, t2 = 0ull;
+    Entry e = {-INFINITY, kNone};
+    float thr_v = -INFINITY, floor_v = -INFINITY;  // the list's num_top-th logit; no logit below floor_v is among the best
+    int thr_i = kNone;
+    auto offer = [&](float v, int i) {  // candidates of all lanes, in any order; i = kNone: none
+        uint32_t who = __ballot_sync(0xffffffffu, v >= floor_v && before(v, i, thr_v, thr_i));
+        while (who) {
+            const int src = __ffs(who) - 1;
+            who &= who - 1;
+            const float nv = __shfl_sync(0xffffffffu, v, src);
+            const int ni = __shfl_sync(0xffffffffu, i, src);
+            if (before(nv, ni, thr_v, thr_i)) {
+                insert(e, nv, ni);
+                thr_v = __shfl_sync(0xffffffffu, e.v, p.num_top - 1);
+                thr_i = __shfl_sync(0xffffffffu, e.i, p.num_top - 1);
+            }
+        }
+    };
+    auto grow = [&](float to) {  // a larger maximum
+        const float d = max_nan(m - to, -1e4f), f = exp2_approx(d * kLog2e);  // (as in rescale; the sums are zero while m is -infinity)
+        const f32x2 f2 = make_x2(f, f), d2 = make_x2(d, d);
+        t2 = mul2(f2, fma2(s2, d2, t2));
+        s2 = mul2(f2, s2);
+        m = to;
+    };
+    auto add_pair = [&](f32x2 v) {
+        const float2 d = split_x2(add2(v, make_x2(-m, -m)));
+        // a forbidden logit's exponential is zero, and its product with the difference has to be: the difference must not be infinite
+        const f32x2 c = make_x2(max_nan(d.x, -1e4f), max_nan(d.y, -1e4f));
+        const float2 a = split_x2(mul2(c, make_x2(kLog2e, kLog2e)));
+        const f32x2 ex = make_x2(exp2_approx(a.x), exp2_approx(a.y));
+        s2 = add2(s2, ex);
+        t2 = fma2(ex, c, t2);
+    };
+
+    bool first = true;
+    for (int base = p0 + (W == 1 ? 0 : warp * 32); base < p1 || (TOP && first); base += kLanes * kU) {
+        Pack<T, VEC> q[kU];
+        float pm[kU], gm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int k = base + u * kLanes + lane;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[u].w[j] = kNegInf;
+            if (k < p1) q[u].load(body + (int64_t)k * VEC);
+        }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            pm[u] = q[u].max_value();
+            gm = max_nan(gm, pm[u]);
+        }
+        if (TOP && first) {
+            float top = sort_lanes(rank_value(gm));
+            if constexpr (W > 1) {
+                maxima[warp][lane] = top;
+                __syncthreads();
+                for (int w = 0; w < kWarps; ++w)
+                    if (w != warp) top = merge_lanes(top, maxima[w][lane]);
+            }
+            floor_v = __shfl_sync(0xffffffffu, top, p.num_top - 1);
+            first = false;
+        }
+        if (!(gm <= m)) grow(gm);
+        if (m != -INFINITY)
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) add_pair(q[u].pair(j));
+        if constexpr (TOP) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int k = base + u * kLanes + lane, i0 = head + k * VEC;
+                const float best = rank_value(pm[u]);
+                if (!__any_sync(0xffffffffu, k < p1 && best >= floor_v && before(best, i0, thr_v, thr_i))) continue;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) offer(rank_value(q[u].get(j)), k < p1 ? i0 + j : kNone);
+            }
+        }
+    }
+    if (rank == 0 && (W == 1 || warp == 0)) {  // the ends of the row, fewer than 32 logits
+        const int i = lane < head ? lane : V - tail + (lane - head);
+        const bool have = lane < head + tail;
+        const float v = have ? to_f32(x[i]) : -INFINITY;
+        if (!(v <= m)) grow(v);
+        if (m != -INFINITY) add_pair(make_x2(v, -INFINITY));
+        if constexpr (TOP) offer(rank_value(v), have ? i : kNone);
+    }
+
+    const float2 ss = split_x2(s2), tt = split_x2(t2);
+    Part a = {m, ss.x + ss.y, tt.x + tt.y};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)});
+    if constexpr (W > 1) {
+        if (lane == 0) parts[warp] = a;
+        if constexpr (TOP) lists[warp][lane] = e;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < kWarps; ++w) {
+                a = join(a, parts[w]);
+                if constexpr (TOP) merge(e, lists[w][lane]);
+            }
+        }
+        if (split > 1) {
+            // (every thread comes to both barriers; the second keeps the blocks' shared memory in place until the first block has read it)
+            __syncwarp();
+            if (warp == 0) {
+                if (lane == 0) parts[0] = a;
+                if constexpr (TOP) lists[0][lane] = e;
+            }
+            tc::cluster_sync_all();
+            if (rank == 0 && warp == 0)
+                for (int c = 1; c < split; ++c) {
+                    Part b;
+                    const uint32_t at = tc::map_to_cta(tc::smem_u32(&parts[0]), c);
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.m) : "r"(at) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.s) : "r"(at + 4) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.t) : "r"(at + 8) : "memory");
+                    a = join(a, b);
+                    if constexpr (TOP) {
+                        Entry o;
+                        const uint32_t le = tc::map_to_cta(tc::smem_u32(&lists[0][lane]), c);
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(o.v) : "r"(le) : "memory");
+                        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(o.i) : "r"(le + 4) : "memory");
+                        merge(e, o);
+                    }
+                }
+            tc::cluster_sync_all();
+        }
+        if (warp != 0 || rank != 0) return;
+    }
+    const bool empty = a.m == -INFINITY;
+    const float log_total = logf(a.s);
+    // log probabilities as (x - m) - log_total, not through their rounded sum
+    if (TOP && lane < p.num_top) {
+        p.top_lp[r * p.num_top + lane] = empty ? -INFINITY : (e.v - a.m) - log_total;
+        p.top_tok[r * p.num_top + lane] = e.i;
+    }
+    if (lane == 0) {
+        const int64_t tok = load_token(p.tokens, p.token_dtype, r);
+        float lp = nanf("");
+        if (p.has_ignore && tok == p.ignore) lp = 0.f;
+        else if (tok >= 0 && tok < V) lp = empty ? -INFINITY : (to_f32(x[tok]) - a.m) - log_total;
+        p.logprob[r] = lp;
+        p.entropy[r] = empty ? 0.f : log_total - a.t / a.s;
+        p.lse[r] = empty ? -INFINITY : a.m + log_total;
+    }
+}
+
+// ---- gradient -------------------------------------------------------------------------------------------------------------
 
 template <typename F>
 __device__ __forceinline__ float block_reduce(float v, float* red, F&& f) {
@@ -33,71 +308,8 @@ __device__ __forceinline__ float block_reduce(float v, float* red, F&& f) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = red[0];
-    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) s = f(s, red[i]);
+    for (int i = 1; i < kWarps; ++i) s = f(s, red[i]);
     return s;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, const void* __restrict__ tokens, int token_dtype,
-                                                                  int64_t rows, int64_t V, int num_top, int has_ignore, int64_t ignore,
-                                                                  float* __restrict__ logprob, float* __restrict__ entropy, float* __restrict__ lse_out,
-                                                                  float* __restrict__ top_lp, int64_t* __restrict__ top_tok) {
-    __shared__ float red[kThreads / 32];
-    __shared__ Best bred[kThreads / 32];
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const T* x = logits + r * ld;
-        float m = -INFINITY;
-        bool nan = false;
-        for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-            const float v = to_f32(x[i]);
-            nan = nan || v != v;
-            m = fmaxf(m, v);
-        }
-        m = block_reduce(nan ? INFINITY : m, red, [](float a, float b) { return fmaxf(a, b); });
-        float s = 0.f, t = 0.f;
-        if (m > -INFINITY)
-            for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-                const float a = to_f32(x[i]) - m, e = expf(a);
-                s += e;
-                t += e == 0.f ? 0.f : e * a;
-            }
-        s = block_reduce(s, red, [](float a, float b) { return a + b; });
-        t = block_reduce(t, red, [](float a, float b) { return a + b; });
-        const bool empty = m == -INFINITY;
-        const float lse = empty ? -INFINITY : m + logf(s);
-        if (threadIdx.x == 0) {
-            const int64_t tok = load_token(tokens, token_dtype, r);
-            float lp = nanf("");
-            if (has_ignore && tok == ignore) lp = 0.f;
-            else if (tok >= 0 && tok < V) lp = empty ? -INFINITY : (to_f32(x[tok]) - m) - logf(s);  // not through lse, which rounds where m is large
-            logprob[r] = lp;
-            entropy[r] = empty ? 0.f : logf(s) - t / s;
-            lse_out[r] = lse;
-        }
-        Best last = {INFINITY, -1};
-        for (int k = 0; k < num_top; ++k) {
-            Best b = {-INFINITY, 0x7fffffff};
-            for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-                const Best c = {rank_value(to_f32(x[i])), (int)i};
-                if (before(last, c) && before(c, b)) b = c;
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const Best c = {__shfl_xor_sync(0xffffffffu, b.v, o), __shfl_xor_sync(0xffffffffu, b.i, o)};
-                if (before(c, b)) b = c;
-            }
-            __syncthreads();
-            if ((threadIdx.x & 31) == 0) bred[threadIdx.x >> 5] = b;
-            __syncthreads();
-            last = bred[0];
-            for (int i = 1; i < kThreads / 32; ++i)
-                if (before(bred[i], last)) last = bred[i];
-            if (threadIdx.x == 0) {
-                top_tok[r * num_top + k] = last.i;
-                top_lp[r * num_top + k] = empty ? -INFINITY : (to_f32(x[last.i]) - m) - logf(s);
-            }
-        }
-    }
 }
 
 // log p = (x - shift) - log_total.  lse is the sum of the two and rounds: from 1024 on by up to 2^-14 and more, and in a row of nothing but the type's
@@ -107,7 +319,8 @@ struct RowScale {
 };
 template <typename T>
 __device__ RowScale row_scale(const T* __restrict__ x, int64_t V, float lse, float* red) {
-    if (!(fabsf(lse) > 1024.f) || fabsf(lse) == INFINITY) return {lse, 0.f};
+    if (lse == -INFINITY) return {0.f, 0.f};  // nothing but forbidden logits: probabilities of zero
+    if (!(fabsf(lse) > 1024.f) || lse == INFINITY) return {lse, 0.f};
     float m = -INFINITY, s = 0.f;
     for (int64_t i = threadIdx.x; i < V; i += blockDim.x) m = fmaxf(m, to_f32(x[i]));
     m = block_reduce(m, red, [](float a, float b) { return fmaxf(a, b); });
@@ -115,23 +328,70 @@ __device__ RowScale row_scale(const T* __restrict__ x, int64_t V, float lse, flo
     return {m, logf(block_reduce(s, red, [](float a, float b) { return a + b; }))};
 }
 
+// A block takes kThreads * kU pieces of sixteen bytes of one row, by where dlogits has them; the logits are read as pieces too where the row starts at
+// the same place of a piece in both, and one by one elsewhere.
+constexpr int kGradU = 4;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) token_logprobs_grad_kernel(const float* __restrict__ dlogprob, const float* __restrict__ dentropy,
                                                                        const T* __restrict__ logits, int64_t ld, const void* __restrict__ tokens, int token_dtype,
-                                                                       const float* __restrict__ lse, const float* __restrict__ entropy, int64_t rows, int64_t V,
-                                                                       int has_ignore, int64_t ignore, T* __restrict__ dlogits) {
-    __shared__ float red[kThreads / 32];
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        const int64_t tok = load_token(tokens, token_dtype, r);
-        const float g = !dlogprob || (has_ignore && tok == ignore) ? 0.f : (tok < 0 || tok >= V ? nanf("") : dlogprob[r]), h = dentropy ? dentropy[r] : 0.f, l = lse[r];
-        const float H = entropy ? entropy[r] : 0.f;
-        const RowScale sc = row_scale(logits + r * ld, V, l, red);
-        for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < V; i += (int64_t)gridDim.x * kThreads) {
-            const float v = to_f32(logits[r * ld + i]);
-            const float a = v == -INFINITY ? -INFINITY : (v - sc.shift) - sc.log_total, p = expf(a);
-            float d = p == 0.f ? 0.f : -p * (g + h * (a + H));
-            if (i == tok) d += g;
-            dlogits[r * V + i] = from_f32<T>(d);
+                                                                       const float* __restrict__ lse, const float* __restrict__ entropy, int V, int chunks, int has_ignore,
+                                                                       int64_t ignore, T* __restrict__ dlogits) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    __shared__ float red[kWarps];
+    pdl_launch_dependents();
+    pdl_dependency_wait();
+    const int64_t r = blockIdx.x / (unsigned)chunks;
+    const int chunk = (int)(blockIdx.x % (unsigned)chunks);
+    const T* x = logits + r * ld;
+    T* out = dlogits + r * V;
+    const int mis = (int)(reinterpret_cast<uintptr_t>(out) & 15u) / (int)sizeof(T);
+    const bool same = (reinterpret_cast<uintptr_t>(out) & 15u) == (reinterpret_cast<uintptr_t>(x) & 15u);
+    const int c0 = (chunk * kThreads * kGradU + (int)threadIdx.x) * VEC - mis;  // first column of the thread's first piece
+    Pack<T, VEC> q[kGradU];
+    auto column = [&](int u) { return c0 + u * kThreads * VEC; };
+    auto full = [&](int u) { return column(u) >= 0 && column(u) + VEC <= V; };
+#pragma unroll
+    for (int u = 0; u < kGradU; ++u) {
+        q[u].zero();
+        if (full(u) && same) q[u].load(x + column(u));
+    }
+    if (!same)
+#pragma unroll
+        for (int u = 0; u < kGradU; ++u)
+            if (full(u))
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) q[u].put(j, x[column(u) + j]);
+    const int64_t tok = load_token(tokens, token_dtype, r);
+    const float g = !dlogprob || (has_ignore && tok == ignore) ? 0.f : (tok < 0 || tok >= V ? nanf("") : dlogprob[r]), h = dentropy ? dentropy[r] : 0.f;
+    const float H = entropy ? entropy[r] : 0.f;
+    const int mine = tok >= 0 && tok < V ? (int)tok : -VEC;  // (never among a thread's columns)
+    const RowScale sc = row_scale(x, V, lse[r], red);
+    const f32x2 ns = make_x2(-sc.shift, -sc.shift), nt = make_x2(-sc.log_total, -sc.log_total), k0 = make_x2(-fmaf(h, H, g), -fmaf(h, H, g)), k1 = make_x2(-h, -h);
+    // -p (g + h (log p + H)) of two logits; log p is kept finite, since its product with a probability of zero has to be zero
+    auto grad = [&](f32x2 v) {
+        const float2 a = split_x2(add2(add2(v, ns), nt));
+        const f32x2 lp = make_x2(max_nan(a.x, -1e4f), max_nan(a.y, -1e4f));
+        const float2 e = split_x2(mul2(lp, make_x2(kLog2e, kLog2e)));
+        return mul2(make_x2(exp2_approx(e.x), exp2_approx(e.y)), fma2(lp, k1, k0));
+    };
+#pragma unroll
+    for (int u = 0; u < kGradU; ++u) {
+        const int c = column(u);
+        if (full(u)) {
+            f32x2 d[VEC / 2];
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) d[j] = grad(q[u].pair(j));
+            if ((unsigned)(mine - c) < (unsigned)VEC)
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) d[j] = add2(d[j], make_x2(mine == c + 2 * j ? g : 0.f, mine == c + 2 * j + 1 ? g : 0.f));
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) q[u].set_pair(j, d[j]);
+            q[u].store(out + c);
+        } else if (c < V && c + VEC > 0) {
+            for (int j = max(0, -c); j < VEC && c + j < V; ++j) {
+                const float d = split_x2(grad(make_x2(to_f32(x[c + j]), 0.f))).x;
+                out[c + j] = from_f32<T>(d + (mine == c + j ? g : 0.f));
+            }
         }
     }
 }
@@ -156,13 +416,25 @@ extern "C" int chxq_token_logprobs(const void* logits, int64_t ld, int32_t dtype
     CHXQ_CHECK_ARG(num_top >= 0 && num_top <= CHXQ_MAX_TOP && num_top <= V, "TokenLogProbs: num_top must be at most %d and at most the number of logits", CHXQ_MAX_TOP);
     if (rows == 0) return CHXQ_OK;
     CHXQ_CHECK_ARG(logits && tokens && logprob && entropy && log_sum_exp && (num_top == 0 || (top_logprobs && top_tokens)), "TokenLogProbs: null argument");
+    const LogprobArgs a = {tokens, token_dtype, num_top, has_ignore, rows, ignore_index, logprob, entropy, log_sum_exp, top_logprobs, top_tokens};
+    cudaStream_t s = as_stream(stream);
     return with_float_type(dtype, [&](auto t) {
         using T = decltype(t);
-        token_logprobs_kernel<T><<<(unsigned)(rows < 148 * 8 ? rows : 148 * 8), kThreads, 0, as_stream(stream)>>>(
-                static_cast<const T*>(logits), ld, tokens, token_dtype, rows, V, num_top, has_ignore, ignore_index, logprob, entropy, log_sum_exp, top_logprobs,
-                top_tokens);
-        CHXQ_LAUNCH_CHECK();
-        return CHXQ_OK;
+        // A warp per row up to 2048 logits where there are rows enough to fill the warps; else a block, or a cluster of them as long as the blocks
+        // do not fill the SMs twice and each still has a round of its accesses.
+        const int round = kThreads * 4 * 16 / (int)sizeof(T);
+        int split = 1;
+        while (split < 8 && rows * split < 2 * 148 && V >= (int64_t)round * split * 2) split *= 2;
+        const bool warps = V <= 2048 && rows >= 148 * 4;
+        const int64_t grid = warps ? (rows + kWarps - 1) / kWarps : rows * split;
+        if (grid >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "TokenLogProbs: too many rows");
+        auto go = [&](auto* kernel) {
+            CHXQ_CUDA(launch_pdl_cluster(split, kernel, dim3((unsigned)grid), kThreads, 0, s, static_cast<const T*>(logits), ld, (int)V, split, a));
+            count_launch(1);
+            return CHXQ_OK;
+        };
+        if (warps) return num_top ? go(token_logprobs_kernel<T, 1, true>) : go(token_logprobs_kernel<T, 1, false>);
+        return num_top ? go(token_logprobs_kernel<T, kWarps, true>) : go(token_logprobs_kernel<T, kWarps, false>);
     });
 }
 
@@ -173,12 +445,16 @@ extern "C" int chxq_token_logprobs_grad(const float* dlogprob, const float* dent
     if (rc != CHXQ_OK) return rc;
     if (rows == 0) return CHXQ_OK;
     CHXQ_CHECK_ARG(logits && tokens && log_sum_exp && dlogits && (!dentropy || entropy), "TokenLogProbsGrad: null argument");
-    const dim3 grid((unsigned)((V + 4 * kThreads - 1) / (4 * kThreads)), (unsigned)(rows < 65535 ? rows : 65535));
+    cudaStream_t s = as_stream(stream);
     return with_float_type(dtype, [&](auto t) {
         using T = decltype(t);
-        token_logprobs_grad_kernel<T><<<grid, kThreads, 0, as_stream(stream)>>>(dlogprob, dentropy, static_cast<const T*>(logits), ld, tokens, token_dtype,
-                                                                                log_sum_exp, entropy, rows, V, has_ignore, ignore_index, static_cast<T*>(dlogits));
-        CHXQ_LAUNCH_CHECK();
+        constexpr int VEC = 16 / (int)sizeof(T);
+        const int64_t per_block = (int64_t)kThreads * kGradU * VEC;
+        const int64_t chunks = (V + VEC - 1 + per_block - 1) / per_block;  // wherever in a piece a row starts
+        if (chunks * rows >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "TokenLogProbsGrad: too many logits");
+        CHXQ_CUDA(launch_pdl(token_logprobs_grad_kernel<T>, dim3((unsigned)(chunks * rows)), kThreads, 0, s, dlogprob, dentropy, static_cast<const T*>(logits), ld, tokens,
+                             (int)token_dtype, log_sum_exp, entropy, (int)V, (int)chunks, (int)has_ignore, ignore_index, static_cast<T*>(dlogits)));
+        count_launch(1);
         return CHXQ_OK;
     });
 }
