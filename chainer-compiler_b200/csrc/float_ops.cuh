@@ -162,6 +162,34 @@ struct Pack {
             return r;
         }
     }
+    // Bit i: value i is not below `bound` (NaN is not), which is a value of T itself.
+    __device__ __forceinline__ uint32_t not_below(float bound) const {
+        uint32_t r = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r |= !(__uint_as_float(w[i]) < bound) ? 1u << i : 0u;
+        } else {
+            const T h = from_f32<T>(bound);
+            const uint32_t b = *reinterpret_cast<const uint16_t*>(&h) * 0x00010001u;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                uint32_t m;  // per half: all ones where it is not below
+                const uint32_t v = w[i];
+                if constexpr (std::is_same<T, __half>::value) m = __hgeu2_mask(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&b));
+                else m = __hgeu2_mask(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&b));
+                r |= ((m & 1u) | (m >> 30 & 2u)) << (2 * i);
+            }
+        }
+        return r;
+    }
+    __device__ __forceinline__ float pick(int i) const {  // value i, where i is not known at compile time
+        static_assert(kWords == 4, "a 16-byte access");
+        const int k = sizeof(T) == 4 ? i : i >> 1;
+        const uint32_t a = k & 1 ? w[1] : w[0], b = k & 1 ? w[3] : w[2], v = k & 2 ? b : a;
+        if constexpr (sizeof(T) == 4) return __uint_as_float(v);
+        const uint16_t h = (uint16_t)(v >> (16 * (i & 1)));
+        return to_f32(*reinterpret_cast<const T*>(&h));
+    }
     __device__ __forceinline__ T value(int i) const {  // as it is stored
         if constexpr (sizeof(T) == 4) {
             return __uint_as_float(w[i]);

@@ -65,14 +65,18 @@ __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) {
 __device__ __forceinline__ float rank_value(float v) {  // NaN ranks with +infinity
     return v != v ? INFINITY : v;
 }
-// Puts (v, i), the same for all lanes, in its place.
-__device__ __forceinline__ void insert(Entry& e, float v, int i) {
+// The lanes' entries in the order of a list.
+__device__ __forceinline__ void sort(Entry& e) {
     const int lane = threadIdx.x & 31;
-    const int pos = __popc(__ballot_sync(0xffffffffu, before(e.v, e.i, v, i)));
-    const float uv = __shfl_up_sync(0xffffffffu, e.v, 1);
-    const int ui = __shfl_up_sync(0xffffffffu, e.i, 1);
-    if (lane > pos) e = {uv, ui};
-    if (lane == pos) e = {v, i};
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            const float v = __shfl_xor_sync(0xffffffffu, e.v, d);
+            const int i = __shfl_xor_sync(0xffffffffu, e.i, d);
+            const bool first = ((lane & size) == 0) == ((lane & d) == 0);  // this lane takes the entry that ranks first
+            if (before(v, i, e.v, e.i) == first) e = {v, i};
+        }
 }
 // The best 32 of two lists: the larger of one and the reversed other is a bitonic sequence of them, which five steps sort.
 __device__ __forceinline__ void merge(Entry& e, Entry o) {
@@ -100,17 +104,6 @@ __device__ __forceinline__ float sort_lanes(float v) {
         }
     return v;
 }
-__device__ __forceinline__ float merge_lanes(float v, float o) {  // the best 32 of two sorted sets of lanes, sorted
-    const int lane = threadIdx.x & 31;
-    v = fmaxf(v, __shfl_sync(0xffffffffu, o, 31 - lane));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const float q = __shfl_xor_sync(0xffffffffu, v, d);
-        v = (lane & d) == 0 ? fmaxf(v, q) : fminf(v, q);
-    }
-    return v;
-}
-
 // ---- forward --------------------------------------------------------------------------------------------------------------
 
 struct LogprobArgs {
@@ -124,16 +117,20 @@ struct LogprobArgs {
 // One pass over a row: the running maximum and the two sums of a thread are rescaled when the maximum grows.  W warps take a row (one for short rows, else
 // the block's eight), or the blocks of a cluster (W = 8) a part of it each; the parts meet in shared memory, and the blocks' in the first block's
 // through distributed shared memory.  A thread has kU accesses of sixteen bytes in flight; up to 15 bytes at either end of a row are read one by one.
-// Alternatives (TOP): a warp keeps its best 32 logits, one per lane.  Few logits get as far as the insertion: after the first round of accesses the num_top-th
-// largest of the threads' maxima bounds the num_top-th best from below, and so does the list itself.
+// Alternatives (TOP): the num_top-th largest of 32 running maxima -- each over the threads of one lane number -- bounds the num_top-th best logit from below.
+// It is taken anew after 1, 4, 16, ... rounds of accesses (1, 2, 4, ... for many alternatives), so that a few times num_top logits are above
+// it; those go into a buffer of their warp, unsorted, and are sorted at the end (or when the buffer is full: ascending rows), 32 at a time.
 // Bound: HBM; per logit one conversion, one maximum, four instructions on pairs, a clamp and an exponential.
 template <typename T, int W, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V, int split, const LogprobArgs p) {
     constexpr int VEC = 16 / (int)sizeof(T), kU = 4;
     constexpr uint32_t kNegInf = sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u);
+    constexpr int kBuffer = 2 * 32 * VEC;  // twice what an access of the warp's lanes may add
     __shared__ Part parts[kWarps];
     __shared__ Entry lists[TOP ? kWarps : 1][32];
-    __shared__ float maxima[TOP ? kWarps : 1][32];
+    __shared__ float maxima[TOP ? 2 : 1][TOP ? kWarps : 1][32];
+    __shared__ Entry buffers[TOP ? kWarps : 1][TOP ? kBuffer : 1];
+    __shared__ int counts[kWarps];
     pdl_launch_dependents();
     pdl_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -153,19 +150,45 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
     Entry e = {-INFINITY, kNone};
     float thr_v = -INFINITY, floor_v = -INFINITY;  // the list's num_top-th logit; no logit below floor_v is among the best
     int thr_i = kNone;
-    auto offer = [&](float v, int i) {  // candidates of all lanes, in any order; i = kNone: none
-        uint32_t who = __ballot_sync(0xffffffffu, v >= floor_v && before(v, i, thr_v, thr_i));
-        while (who) {
-            const int src = __ffs(who) - 1;
-            who &= who - 1;
-            const float nv = __shfl_sync(0xffffffffu, v, src);
-            const int ni = __shfl_sync(0xffffffffu, i, src);
-            if (before(nv, ni, thr_v, thr_i)) {
-                insert(e, nv, ni);
-                thr_v = __shfl_sync(0xffffffffu, e.v, p.num_top - 1);
-                thr_i = __shfl_sync(0xffffffffu, e.i, p.num_top - 1);
+    if (TOP && lane == 0) counts[warp] = 0;
+    __syncwarp();
+    // Sorts the warp's buffer into its list.
+    bool listed = false;
+    auto settle = [&]() {
+        __syncwarp();
+        const int n = counts[warp];
+        for (int c = 0; c < n; c += 32) {
+            Entry o = {-INFINITY, kNone};
+            if (c + lane < n) o = buffers[warp][c + lane];
+            sort(o);
+            if (listed) merge(e, o);
+            else e = o;
+            listed = true;
+        }
+        __syncwarp();
+        if (lane == 0) counts[warp] = 0;
+        __syncwarp();
+        thr_v = __shfl_sync(0xffffffffu, e.v, p.num_top - 1);
+        thr_i = __shfl_sync(0xffffffffu, e.i, p.num_top - 1);
+    };
+    // The lane's candidates -- value(j) at index i0 + j for every bit j of `which` -- go to the buffer; all lanes take part.  Once there is a list, equal
+    // logits behind its num_top-th are turned away (in a row of one value, all of them).
+    auto offer = [&](const auto& value, uint32_t which, int i0) __attribute__((always_inline)) {
+        if (listed) {
+            for (uint32_t w = which; w; w &= w - 1) {
+                const int j = __ffs(w) - 1;
+                if (!before(rank_value(value(j)), i0 + j, thr_v, thr_i)) which &= ~(1u << j);
             }
         }
+        if (which) {
+            int at = atomicAdd(&counts[warp], __popc(which));  // (any order: they are sorted later, and no two are equal)
+            for (; which; which &= which - 1) {
+                const int j = __ffs(which) - 1;
+                buffers[warp][at++] = {rank_value(value(j)), i0 + j};
+            }
+        }
+        __syncwarp();
+        if (counts[warp] > kBuffer / 2) settle();
     };
     auto grow = [&](float to) {  // a larger maximum
         const float d = max_nan(m - to, -1e4f), f = exp2_approx(d * kLog2e);  // (as in rescale; the sums are zero while m is -infinity)
@@ -184,10 +207,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
         t2 = fma2(ex, c, t2);
     };
 
-    bool first = true;
-    for (int base = p0 + (W == 1 ? 0 : warp * 32); base < p1 || (TOP && first); base += kLanes * kU) {
-        Pack<T, VEC> q[kU];
+    const int rounds = (p1 - p0 + kLanes * kU - 1) / (kLanes * kU);
+    int update = 0, par = 0;
+    for (int round = 0; round < rounds; ++round) {
+        const int base = p0 + round * kLanes * kU + (W == 1 ? 0 : warp * 32);
         float pm[kU], gm = -INFINITY;
+        Pack<T, VEC> q[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int k = base + u * kLanes + lane;
@@ -200,31 +225,31 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
             pm[u] = q[u].max_value();
             gm = max_nan(gm, pm[u]);
         }
-        if (TOP && first) {
-            float top = sort_lanes(rank_value(gm));
-            if constexpr (W > 1) {
-                maxima[warp][lane] = top;
-                __syncthreads();
-                for (int w = 0; w < kWarps; ++w)
-                    if (w != warp) top = merge_lanes(top, maxima[w][lane]);
-            }
-            floor_v = __shfl_sync(0xffffffffu, top, p.num_top - 1);
-            first = false;
-        }
         if (!(gm <= m)) grow(gm);
+        if (TOP && round == update) {
+            update = p.num_top > 8 ? 2 * update + 1 : 4 * update + 3;
+            float top = rank_value(m);
+            if constexpr (W > 1) {
+                maxima[par][warp][lane] = top;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, maxima[par][w][lane]);
+                par ^= 1;  // (the maxima of two updates ago have been read by all when these are overwritten)
+            }
+            floor_v = __shfl_sync(0xffffffffu, sort_lanes(top), p.num_top - 1);
+        }
         if (m != -INFINITY)
 #pragma unroll
             for (int u = 0; u < kU; ++u)
 #pragma unroll
                 for (int j = 0; j < VEC / 2; ++j) add_pair(q[u].pair(j));
-        if constexpr (TOP) {
+        if (TOP && __any_sync(0xffffffffu, !(gm < floor_v))) {  // (NaN passes, too)
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-                const int k = base + u * kLanes + lane, i0 = head + k * VEC;
-                const float best = rank_value(pm[u]);
-                if (!__any_sync(0xffffffffu, k < p1 && best >= floor_v && before(best, i0, thr_v, thr_i))) continue;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) offer(rank_value(q[u].get(j)), k < p1 ? i0 + j : kNone);
+                const int k = base + u * kLanes + lane;
+                const bool some = k < p1 && !(pm[u] < floor_v);
+                if (!__any_sync(0xffffffffu, some)) continue;
+                offer([&](int j) { return q[u].pick(j); }, some ? q[u].not_below(floor_v) : 0u, head + k * VEC);
             }
         }
     }
@@ -234,8 +259,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
         const float v = have ? to_f32(x[i]) : -INFINITY;
         if (!(v <= m)) grow(v);
         if (m != -INFINITY) add_pair(make_x2(v, -INFINITY));
-        if constexpr (TOP) offer(rank_value(v), have ? i : kNone);
+        if constexpr (TOP) offer([&](int) { return v; }, have && !(v < floor_v) ? 1u : 0u, i);
     }
+    if constexpr (TOP) settle();
 
     const float2 ss = split_x2(s2), tt = split_x2(t2);
     Part a = {m, ss.x + ss.y, tt.x + tt.y};
@@ -243,13 +269,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
     for (int o = 16; o > 0; o >>= 1)
         a = join(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)});
     if constexpr (W > 1) {
-        if (lane == 0) parts[warp] = a;
-        if constexpr (TOP) lists[warp][lane] = e;
-        __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < kWarps; ++w) {
-                a = join(a, parts[w]);
-                if constexpr (TOP) merge(e, lists[w][lane]);
+        for (int d = kWarps / 2; d > 0; d >>= 1) {  // the upper half of the warps hands its part to the lower
+            if (warp >= d && warp < 2 * d) {
+                if (lane == 0) parts[warp] = a;
+                if constexpr (TOP) lists[warp][lane] = e;
+            }
+            __syncthreads();
+            if (warp < d) {
+                a = join(a, parts[warp + d]);
+                if constexpr (TOP) merge(e, lists[warp + d][lane]);
             }
         }
         if (split > 1) {
@@ -420,12 +448,12 @@ extern "C" int chxq_token_logprobs(const void* logits, int64_t ld, int32_t dtype
     cudaStream_t s = as_stream(stream);
     return with_float_type(dtype, [&](auto t) {
         using T = decltype(t);
-        // A warp per row up to 2048 logits where there are rows enough to fill the warps; else a block, or a cluster of them as long as the blocks
+        // A warp per row where there are rows enough for half of the warps that fit; else a block, or a cluster of them as long as the blocks
         // do not fill the SMs twice and each still has a round of its accesses.
         const int round = kThreads * 4 * 16 / (int)sizeof(T);
         int split = 1;
         while (split < 8 && rows * split < 2 * 148 && V >= (int64_t)round * split * 2) split *= 2;
-        const bool warps = V <= 2048 && rows >= 148 * 4;
+        const bool warps = V <= 16384 && rows >= 148 * 8;
         const int64_t grid = warps ? (rows + kWarps - 1) / kWarps : rows * split;
         if (grid >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "TokenLogProbs: too many rows");
         auto go = [&](auto* kernel) {
