@@ -1,8 +1,8 @@
 // Linear with bias, activation and residual in its epilogue: y = act(x w^T + b) + r, or act(x w^T + b + r); bf16, fp16 and fp32 operands,
 // sums in 32 bits, one rounding at the end.
 //
-// Three kernels: CTA pairs with 256 x 256 blocks (linear_pair.cuh) for large 16-bit products, clusters that share a tile's K (linear_tile.cuh) for
-// few rows of x and products in between, and a general CUDA-core kernel.
+// Two kernels: CTA pairs with 256 x 256 blocks (linear_pair.cuh) for large 16-bit products, and clusters that share a tile's K (linear_tile.cuh) for
+// few rows of x, for products in between and for fp32.
 #include <algorithm>
 #include <atomic>
 
@@ -14,91 +14,96 @@
 namespace chxq {
 namespace {
 
-// General kernel: 64 x 64 outputs a block, 4 x 4 a thread, operands through shared memory in 32 bits.  Any extent, row pitch and alignment.
-constexpr int kTile = 64, kSlice = 16;
-
+// Products without a K: the epilogue of sums of zero.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_simt_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int64_t M, int64_t O,
-                                                          int64_t K, LinearEpilogue e) {
-    __shared__ float xs[kSlice][kTile + 1], ws[kSlice][kTile + 1];
-    const int tid = threadIdx.x;
-    const int64_t m0 = (int64_t)blockIdx.y * kTile, o0 = (int64_t)blockIdx.x * kTile;
-    const int tm = tid / 16, to = tid % 16;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += kSlice) {
-#pragma unroll
-        for (int i = 0; i < kTile * kSlice / 256; ++i) {
-            const int f = tid + 256 * i, r = f / kSlice, k = f % kSlice;
-            const bool in = k0 + k < K;
-            xs[k][r] = in && m0 + r < M ? to_f32(x[(m0 + r) * ldx + k0 + k]) : 0.f;
-            ws[k][r] = in && o0 + r < O ? to_f32(w[(o0 + r) * ldw + k0 + k]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kSlice; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(xs[k][tm * 4 + i], ws[k][to + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + tm * 4 + i, o = o0 + to + 16 * j;
-            if (m < M && o < O) epilogue_store<T>(e, m, o, acc[i][j]);
-        }
+__global__ void __launch_bounds__(256) linear_empty_kernel(int64_t M, int64_t O, LinearEpilogue e) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * O; i += (int64_t)gridDim.x * 256) epilogue_store<T>(e, i / O, i % O, 0.f);
 }
 
 // ---- the tensor-core kernels ------------------------------------------------------------------------------------------------
 
 // TMA reads rows that start on 16-byte boundaries.  Operands whose rows do not are copied into such rows in front of the product.
-bool rows16(const void* p, int64_t ld, int64_t rows) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || ld % 8 == 0);
+bool rows16(const void* p, int64_t ld, int64_t rows, int size) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || ld * size % 16 == 0);
 }
-int64_t pitch16(int64_t K) {
-    return (K + 7) / 8 * 8;
+int64_t pitch16(int64_t K, int size) {
+    const int per = 16 / size;
+    return (K + per - 1) / per * per;
 }
 size_t align256(size_t v) {
     return (v + 255) / 256 * 256;
 }
 
 struct CopyJob {
-    const uint16_t* src;
+    const void* src;
     int64_t ld, rows;
-    uint16_t* dst;
+    void* dst;
 };
 
-// Rows of K 16-bit values into rows of `pitch`, a multiple of 8: a thread gathers eight values and writes them as 16 bytes.  (The last
-// group's values past K are never read: the tensor map ends at K.)
+// Rows of K values into rows of `pitch`, whole 16-byte pieces: a thread gathers one piece.  (The last one's values past K are never read: the tensor map ends
+// at K.)  U: uint16_t or uint32_t.
+template <typename U>
 __global__ void __launch_bounds__(256) align_rows_kernel(CopyJob a, CopyJob b, int64_t K, int64_t pitch) {
+    constexpr int kPer = 16 / (int)sizeof(U);
     pdl_launch_dependents();
     pdl_dependency_wait();
-    const int64_t per_row = pitch / 8, total = (a.rows + b.rows) * per_row;
+    const int64_t per_row = pitch / kPer, total = (a.rows + b.rows) * per_row;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         int64_t r = i / per_row;
-        const int64_t k = (i - r * per_row) * 8;
+        const int64_t k = (i - r * per_row) * kPer;
         const bool first = r < a.rows;
         if (!first) r -= a.rows;
-        const uint16_t* s = (first ? a.src + r * a.ld : b.src + r * b.ld) + k;
+        const U* s = (first ? static_cast<const U*>(a.src) + r * a.ld : static_cast<const U*>(b.src) + r * b.ld) + k;
+        U v[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] = k + j < K ? s[j] : (U)0;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = (k + 2 * j < K ? s[2 * j] : 0u) | ((k + 2 * j + 1 < K ? (uint32_t)s[2 * j + 1] : 0u) << 16);
-        *reinterpret_cast<uint4*>((first ? a.dst + r * pitch : b.dst + r * pitch) + k) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int j = 0; j < 4; ++j) w[j] = sizeof(U) == 4 ? (uint32_t)v[j % kPer] : (uint32_t)v[2 * j % kPer] | (uint32_t)v[(2 * j + 1) % kPer] << 16;
+        *reinterpret_cast<uint4*>((first ? static_cast<U*>(a.dst) : static_cast<U*>(b.dst)) + r * pitch + k) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-// Sets a kernel's dynamic shared memory once per device.
-template <typename F>
-int set_smem(F* kernel, int bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    CHXQ_CUDA(cudaGetDevice(&dev));
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
-    if (done.load(std::memory_order_acquire) & bit) return CHXQ_OK;
-    CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done.fetch_or(bit, std::memory_order_release);
+// What is known of a kernel on each device: whether its dynamic shared memory is set, and how many of its clusters of 1 .. 8 CTAs are resident at once
+// (0: not asked yet).
+struct KernelState {
+    std::atomic<bool> smem_set[64];
+    std::atomic<int> slots[64][9];
+};
+
+int current_device(int* dev) {
+    CHXQ_CUDA(cudaGetDevice(dev));
+    if (*dev < 0 || *dev >= 64) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: device number %d", *dev);
     return CHXQ_OK;
+}
+
+template <typename F>
+int set_smem(F* kernel, int bytes, KernelState& st, int dev) {
+    if (st.smem_set[dev].load(std::memory_order_acquire)) return CHXQ_OK;
+    CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    st.smem_set[dev].store(true, std::memory_order_release);
+    return CHXQ_OK;
+}
+
+template <typename F>
+int cluster_slots(F* kernel, int cluster, int threads, int smem, KernelState& st, int dev) {
+    int n = st.slots[dev][cluster].load(std::memory_order_acquire);
+    if (n > 0) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cluster * 148));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = std::max(1, 100 / cluster);
+    }
+    st.slots[dev][cluster].store(n, std::memory_order_release);
+    return n;
 }
 
 struct Operands {  // as TMA reads them
@@ -108,39 +113,62 @@ struct Operands {  // as TMA reads them
     int64_t ldw;
 };
 
-template <typename T, int BN, int STAGES>
-int launch_tile(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
-    using Cfg = lin::TileConfig<BN, STAGES>;
-    static std::atomic<uint64_t> done{0};
-    auto* kernel = lin::linear_tile_kernel<T, BN, STAGES>;
-    int rc = set_smem(kernel, Cfg::kSmem, done);
-    if (rc != CHXQ_OK) return rc;
+// kernel: one of linear_tile.cuh's, for bn rows of x.
+template <typename F>
+int launch_tile(F* kernel, int bn, int threads, int smem, KernelState& st, const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, int size,
+                cudaStream_t s) {
+    int dev = 0, rc = current_device(&dev);
+    if (rc != CHXQ_OK || (rc = set_smem(kernel, smem, st, dev)) != CHXQ_OK) return rc;
     alignas(64) CUtensorMap tmW, tmX;
-    if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * 2, q.O, op.ldw * 2, 128)) != CHXQ_OK) return rc;
-    if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * 2, q.M, op.ldx * 2, BN)) != CHXQ_OK) return rc;
-    const int64_t x_tiles = (q.M + BN - 1) / BN, tiles = x_tiles * ((q.O + 127) / 128);
+    if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * size, q.O, op.ldw * size, 128)) != CHXQ_OK) return rc;
+    if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * size, q.M, op.ldx * size, bn)) != CHXQ_OK) return rc;
+    const int64_t x_tiles = (q.M + bn - 1) / bn, tiles = x_tiles * ((q.O + 127) / 128);
+    // How many CTAs share a tile: what gives the fewest K blocks one after the other, a wave of clusters costing about kWave of them beside its own (launch,
+    // first loads, joining the sums).  Clusters that do not all fit at once are worth less than smaller ones that do: [256, 2048] x [1000, 2048]^T
+    // in fp32 has 16 tiles, of which the GPU holds 14 or so as clusters of eight, and takes 30 us that way and 15 as clusters of four.
+    constexpr int64_t kWave = 6;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * tc::sm_count() && split * 2 <= args.k_blocks) split *= 2;
+    int64_t best = INT64_MAX;
+    for (int c = 1; c <= 8 && c <= args.k_blocks; ++c) {
+        const int64_t slots = cluster_slots(kernel, c, threads, smem, st, dev);
+        const int64_t cost = (tiles + slots - 1) / slots * ((args.k_blocks + c - 1) / c + kWave);
+        if (cost < best) {
+            best = cost;
+            split = c;
+        }
+    }
     if (tiles * split >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: too many tiles");
-    CHXQ_CUDA(launch_pdl_cluster(split, kernel, dim3((unsigned)(tiles * split)), 256, Cfg::kSmem, s, tmW, tmX, args, split, (int)x_tiles));
+    CHXQ_CUDA(launch_pdl_cluster(split, kernel, dim3((unsigned)(tiles * split)), threads, smem, s, tmW, tmX, args, split, (int)x_tiles));
     count_launch(1);
     return CHXQ_OK;
+}
+
+template <typename T, int BN, int STAGES>
+int launch_tile_16(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
+    static KernelState state = {};
+    return launch_tile(lin::linear_tile_kernel<T, BN, STAGES>, BN, 256, lin::TileConfig<BN, STAGES>::kSmem, state, q, op, args, 2, s);
+}
+
+template <int BN, int STAGES>
+int launch_tile_32(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
+    static KernelState state = {};
+    return launch_tile(lin::linear_tile_f32_kernel<BN, STAGES>, BN, 640, lin::TileF32Config<BN, STAGES>::kSmem, state, q, op, args, 4, s);
 }
 
 template <typename T>
 int launch_pair(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
     using Cfg = lin::PairConfig;
-    static std::atomic<uint64_t> done{0};
+    static KernelState state = {};
     auto* kernel = lin::linear_pair_kernel<T>;
-    int rc = set_smem(kernel, Cfg::kSmem, done);
-    if (rc != CHXQ_OK) return rc;
+    int dev = 0, rc = current_device(&dev);
+    if (rc != CHXQ_OK || (rc = set_smem(kernel, Cfg::kSmem, state, dev)) != CHXQ_OK) return rc;
     lin::PairArgs a;
     a.t = args;
     const int64_t mb = (q.M + 255) / 256, ob = (q.O + 255) / 256;
     if (mb * ob >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: too many blocks");
     a.m_blocks = (int)mb;
     a.o_blocks = (int)ob;
-    a.tma_out = rows16(q.y, q.ldy, q.M);
+    a.tma_out = rows16(q.y, q.ldy, q.M, 2);
     alignas(64) CUtensorMap tmX, tmW, tmY;
     if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * 2, q.M, op.ldx * 2, 128)) != CHXQ_OK) return rc;
     if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * 2, q.O, op.ldw * 2, 128)) != CHXQ_OK) return rc;
@@ -156,10 +184,18 @@ template <typename T>
 int launch_tc(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
     const int64_t blocks = ((q.M + 255) / 256) * ((q.O + 255) / 256);
     if (q.M > 128 && blocks >= tc::sm_count() / 4) return launch_pair<T>(q, op, args, s);
-    if (q.M <= 16) return launch_tile<T, 16, 6>(q, op, args, s);
-    if (q.M <= 32) return launch_tile<T, 32, 5>(q, op, args, s);
-    if (q.M <= 64) return launch_tile<T, 64, 4>(q, op, args, s);
-    return launch_tile<T, 128, 3>(q, op, args, s);
+    if (q.M <= 16) return launch_tile_16<T, 16, 6>(q, op, args, s);
+    if (q.M <= 32) return launch_tile_16<T, 32, 5>(q, op, args, s);
+    if (q.M <= 64) return launch_tile_16<T, 64, 4>(q, op, args, s);
+    return launch_tile_16<T, 128, 3>(q, op, args, s);
+}
+
+template <>
+int launch_tc<float>(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
+    if (q.M <= 16) return launch_tile_32<16, 4>(q, op, args, s);
+    if (q.M <= 32) return launch_tile_32<32, 4>(q, op, args, s);
+    if (q.M <= 64) return launch_tile_32<64, 4>(q, op, args, s);
+    return launch_tile_32<128, 3>(q, op, args, s);
 }
 
 }  // namespace
@@ -181,16 +217,12 @@ static int check_linear(const chxq_linear_params* p) {
     return CHXQ_OK;
 }
 
-// 16-bit operands with a K go to the tensor cores.
-static bool tensor_cores(const chxq_linear_params& p) {
-    return p.dtype != CHXQ_FLOAT32 && p.K > 0;
-}
-
 extern "C" size_t chxq_linear_workspace(const chxq_linear_params* p) {
-    if (!p || !tensor_cores(*p) || p->M <= 0 || p->O <= 0) return 0;
+    if (!p || !is_float_type(p->dtype) || p->K <= 0 || p->M <= 0 || p->O <= 0) return 0;
+    const int size = float_size(p->dtype);
     size_t n = 0;
-    if (!rows16(p->x, p->ldx, p->M)) n += align256((size_t)(p->M * pitch16(p->K)) * 2);
-    if (!rows16(p->w, p->ldw, p->O)) n += align256((size_t)(p->O * pitch16(p->K)) * 2);
+    if (!rows16(p->x, p->ldx, p->M, size)) n += align256((size_t)(p->M * pitch16(p->K, size)) * size);
+    if (!rows16(p->w, p->ldw, p->O, size)) n += align256((size_t)(p->O * pitch16(p->K, size)) * size);
     return n;
 }
 
@@ -203,47 +235,43 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     CHXQ_CHECK_ARG(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "Linear: the workspace must be 256-byte aligned");
     const LinearEpilogue e = {p->bias, p->bias_dtype, p->residual, p->ldr, p->activation, p->residual_first, p->y, p->ldy};
     cudaStream_t s = as_stream(stream);
-    if (tensor_cores(*p)) {
-        Operands op = {p->x, p->ldx, p->w, p->ldw};
-        if (need) {
-            const int64_t pitch = pitch16(p->K);
-            CopyJob jx = {static_cast<const uint16_t*>(p->x), p->ldx, 0, nullptr}, jw = {static_cast<const uint16_t*>(p->w), p->ldw, 0, nullptr};
-            uint8_t* ws = static_cast<uint8_t*>(workspace);
-            if (!rows16(p->x, p->ldx, p->M)) {
-                jx.rows = p->M;
-                jx.dst = reinterpret_cast<uint16_t*>(ws);
-                ws += align256((size_t)(p->M * pitch) * 2);
-                op.x = jx.dst;
-                op.ldx = pitch;
-            }
-            if (!rows16(p->w, p->ldw, p->O)) {
-                jw.rows = p->O;
-                jw.dst = reinterpret_cast<uint16_t*>(ws);
-                op.w = jw.dst;
-                op.ldw = pitch;
-            }
-            const int64_t blocks = ((jx.rows + jw.rows) * (pitch / 8) + 255) / 256;
-            CHXQ_CUDA(launch_pdl(align_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 148 * 16)), 256, 0, s, jx, jw, p->K, pitch));
-            count_launch(1);
+    if (p->K == 0)
+        return with_float_type(p->dtype, [&](auto t) {
+            linear_empty_kernel<decltype(t)><<<(unsigned)std::min<int64_t>((p->M * p->O + 255) / 256, 148 * 8), 256, 0, s>>>(p->M, p->O, e);
+            CHXQ_LAUNCH_CHECK();
+            return CHXQ_OK;
+        });
+    const int size = float_size(p->dtype);
+    Operands op = {p->x, p->ldx, p->w, p->ldw};
+    if (need) {
+        const int64_t pitch = pitch16(p->K, size);
+        CopyJob jx = {p->x, p->ldx, 0, nullptr}, jw = {p->w, p->ldw, 0, nullptr};
+        uint8_t* ws = static_cast<uint8_t*>(workspace);
+        if (!rows16(p->x, p->ldx, p->M, size)) {
+            jx.rows = p->M;
+            op.x = jx.dst = ws;
+            op.ldx = pitch;
+            ws += align256((size_t)(p->M * pitch) * size);
         }
-        lin::TcArgs a;
-        a.M = (int)p->M;
-        a.O = (int)p->O;
-        a.k_blocks = (int)((p->K + 63) / 64);
-        a.idesc = lin::idesc_f16(p->dtype == CHXQ_BFLOAT16 ? lin::kBf16 : lin::kF16);
-        a.e = e;
-        a.vec = rows16(p->y, p->ldy, p->M) && p->O % 8 == 0 && (!p->residual || rows16(p->residual, p->ldr, p->M));
-        a.status = device_status_ptr();
-        if (!a.status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
-        a.wait_limit_ns = (unsigned long long)tc::wait_limit_ns_value();
-        return p->dtype == CHXQ_BFLOAT16 ? launch_tc<__nv_bfloat16>(*p, op, a, s) : launch_tc<__half>(*p, op, a, s);
+        if (!rows16(p->w, p->ldw, p->O, size)) {
+            jw.rows = p->O;
+            op.w = jw.dst = ws;
+            op.ldw = pitch;
+        }
+        const int64_t blocks = ((jx.rows + jw.rows) * (pitch * size / 16) + 255) / 256;
+        CHXQ_CUDA(launch_pdl(size == 4 ? align_rows_kernel<uint32_t> : align_rows_kernel<uint16_t>, dim3((unsigned)std::min<int64_t>(blocks, 148 * 16)), 256, 0, s, jx, jw,
+                             p->K, pitch));
+        count_launch(1);
     }
-    const dim3 grid((unsigned)((p->O + kTile - 1) / kTile), (unsigned)((p->M + kTile - 1) / kTile));
-    if (grid.y > 65535) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: too many rows");
-    return with_float_type(p->dtype, [&](auto t) {
-        using T = decltype(t);
-        linear_simt_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(p->x), p->ldx, static_cast<const T*>(p->w), p->ldw, p->M, p->O, p->K, e);
-        CHXQ_LAUNCH_CHECK();
-        return CHXQ_OK;
-    });
+    lin::TcArgs a;
+    a.M = (int)p->M;
+    a.O = (int)p->O;
+    a.k_blocks = (int)((p->K * size + 127) / 128);
+    a.idesc = lin::idesc_f16(p->dtype == CHXQ_BFLOAT16 ? lin::kBf16 : lin::kF16);  // (fp32 has its own)
+    a.e = e;
+    a.vec = rows16(p->y, p->ldy, p->M, size) && p->O * size % 16 == 0 && (!p->residual || rows16(p->residual, p->ldr, p->M, size));
+    a.status = device_status_ptr();
+    if (!a.status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
+    a.wait_limit_ns = (unsigned long long)tc::wait_limit_ns_value();
+    return with_float_type(p->dtype, [&](auto t) { return launch_tc<decltype(t)>(*p, op, a, s); });
 }

@@ -26,6 +26,70 @@ struct TileConfig {
     static_assert(kSmem <= 227 * 1024, "shared memory over the per-CTA limit");
 };
 
+// From the shares of a tile, [BN][128] sums in the shared memory of each CTA of the cluster, to the outputs of this CTA's rows of x: the shares added in
+// ascending order (the same bits on every run), then bias, activation and residual.  `warp`: this one of WARPS.
+template <typename T, int BN, int WARPS>
+__device__ __forceinline__ void tile_epilogue(const TcArgs& p, const float* sums, int x0, int w0, int rank, int split, int warp, int lane) {
+    constexpr bool kFast = sizeof(T) == 2;
+    const int cols = (BN + split - 1) / split;  // rows of x of this CTA
+    const bool vec = p.vec != 0;
+    auto feature = [&](int j) { return vec ? 4 * lane + j : lane + 32 * j; };
+    float bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bias[j] = p.e.bias && w0 + feature(j) < p.O ? load_param({p.e.bias, p.e.bias_dtype}, w0 + feature(j)) : 0.f;
+    const uint32_t sums0 = smem_u32(sums);
+    for (int c = rank * cols + warp; c < (rank + 1) * cols && c < BN && x0 + c < p.M; c += WARPS) {
+        const int64_t m = x0 + c;
+        float v[4] = {}, res[4] = {};
+        if (vec) {
+            if (w0 + 4 * lane >= p.O) continue;
+            for (int s = 0; s < split; ++s) {
+                float4 q;
+                const uint32_t at = sums0 + (uint32_t)(c * 128 + 4 * lane) * 4u;
+                if (split > 1)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(map_to_cta(at, s)));
+                else
+                    q = *reinterpret_cast<const float4*>(sums + c * 128 + 4 * lane);
+                v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+            }
+            const T* pr = static_cast<const T*>(p.e.residual) + m * p.e.ldr + w0 + 4 * lane;
+            T* py = static_cast<T*>(p.e.y) + m * p.e.ldy + w0 + 4 * lane;
+            if constexpr (sizeof(T) == 4) {
+                if (p.e.residual) {
+                    const float4 q = *reinterpret_cast<const float4*>(pr);
+                    res[0] = q.x; res[1] = q.y; res[2] = q.z; res[3] = q.w;
+                }
+                epilogue_apply<4, kFast>(p.e, v, bias, res);
+                *reinterpret_cast<float4*>(py) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                if (p.e.residual) {
+                    const uint2 q = *reinterpret_cast<const uint2*>(pr);
+                    const float2 lo = unpack16<T>(q.x), hi = unpack16<T>(q.y);
+                    res[0] = lo.x; res[1] = lo.y; res[2] = hi.x; res[3] = hi.y;
+                }
+                epilogue_apply<4, kFast>(p.e, v, bias, res);
+                *reinterpret_cast<uint2*>(py) = make_uint2(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int f = feature(j);
+                for (int s = 0; s < split; ++s) {
+                    float q;
+                    if (split > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(map_to_cta(sums0 + (uint32_t)(c * 128 + f) * 4u, s)));
+                    else q = sums[c * 128 + f];
+                    v[j] += q;
+                }
+                if (p.e.residual && w0 + f < p.O) res[j] = to_f32(static_cast<const T*>(p.e.residual)[m * p.e.ldr + w0 + f]);
+            }
+            epilogue_apply<4, kFast>(p.e, v, bias, res);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (w0 + feature(j) < p.O) static_cast<T*>(p.e.y)[m * p.e.ldy + w0 + feature(j)] = from_f32<T>(v[j]);
+        }
+    }
+}
+
 template <typename T, int BN, int STAGES>
 __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const TcArgs p, int split,
                                                           int x_tiles) {
@@ -115,54 +179,7 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant_
     tc_fence_before();
     if (split > 1) cluster_sync_all();
     else __syncthreads();
-    if (got) {
-        const int cols = (BN + split - 1) / split;  // rows of x of this CTA
-        const bool vec = p.vec != 0;
-        auto feature = [&](int j) { return vec ? 4 * lane + j : lane + 32 * j; };
-        float bias[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bias[j] = p.e.bias && w0 + feature(j) < p.O ? load_param({p.e.bias, p.e.bias_dtype}, w0 + feature(j)) : 0.f;
-        const uint32_t sums0 = smem_u32(sums);
-        for (int c = rank * cols + warp; c < (rank + 1) * cols && c < BN && x0 + c < p.M; c += 8) {
-            const int64_t m = x0 + c;
-            float v[4] = {}, res[4] = {};
-            if (vec) {
-                if (w0 + 4 * lane >= p.O) continue;
-                for (int s = 0; s < split; ++s) {
-                    float4 q;
-                    const uint32_t at = sums0 + (uint32_t)(c * 128 + 4 * lane) * 4u;
-                    if (split > 1)
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(map_to_cta(at, s)));
-                    else
-                        q = *reinterpret_cast<const float4*>(sums + c * 128 + 4 * lane);
-                    v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
-                }
-                if (p.e.residual) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.e.residual) + m * p.e.ldr + w0 + 4 * lane);
-                    const float2 lo = unpack16<T>(q.x), hi = unpack16<T>(q.y);
-                    res[0] = lo.x; res[1] = lo.y; res[2] = hi.x; res[3] = hi.y;
-                }
-                epilogue_apply<4, true>(p.e, v, bias, res);
-                *reinterpret_cast<uint2*>(static_cast<T*>(p.e.y) + m * p.e.ldy + w0 + 4 * lane) = make_uint2(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int f = feature(j);
-                    for (int s = 0; s < split; ++s) {
-                        float q;
-                        if (split > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(map_to_cta(sums0 + (uint32_t)(c * 128 + f) * 4u, s)));
-                        else q = sums[c * 128 + f];
-                        v[j] += q;
-                    }
-                    if (p.e.residual && w0 + f < p.O) res[j] = to_f32(static_cast<const T*>(p.e.residual)[m * p.e.ldr + w0 + f]);
-                }
-                epilogue_apply<4, true>(p.e, v, bias, res);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (w0 + feature(j) < p.O) static_cast<T*>(p.e.y)[m * p.e.ldy + w0 + feature(j)] = from_f32<T>(v[j]);
-            }
-        }
-    }
+    if (got) tile_epilogue<T, BN, 8>(p, sums, x0, w0, rank, split, warp, lane);
     __syncthreads();
     if (*abort_flag) {  // copies in flight get the time to land
         const uint64_t t0 = global_timer_ns();
@@ -170,6 +187,222 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant_
         __syncthreads();
     }
     if (split > 1) cluster_sync_all();  // the others may still be reading this CTA's sums
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Cfg::kTmemCols);
+    }
+}
+
+// ---- fp32 operands ---------------------------------------------------------------------------------------------------------
+//
+// The tensor cores multiply tf32, eleven significant bits.  A value is split as a = h + l with h = tf32(a) and l = tf32(a - h), rounded to nearest, and the
+// product taken as h h' + h l' + l h': what is left out is below 2^-21 |a a'|, the rounding of an fp32 product in a sum of a few.
+// The sums: h h' goes through TMEM in chains of kChain K blocks (at most 32 instructions, whose additions the tensor core may truncate), each then
+// added in registers; the two small products have an accumulator of their own, 2^-11 in size, for the whole of K.
+// Roles as above, with 640 threads: warps 0 and 2 load, warp 1 issues, warps 4-19 split each stage as it arrives (h in place, l beside it; the swizzle does
+// not matter to an elementwise pass), drain the chains and run the epilogue.
+// Bound: the instructions of the splitting (twenty-six per sixteen bytes; with eight warps their latency: 163 us for 2048^3) and shared memory.
+template <int BN, int STAGES>
+struct TileF32Config {
+    static constexpr int kTileW = 128 * 128, kTileX = BN * 128, kRaw = kTileW + kTileX, kStage = 2 * kRaw;
+    static constexpr int kSums = BN * 128 * 4;
+    static constexpr int kData = STAGES * kStage > kSums ? STAGES * kStage : kSums;
+    static constexpr int kNumBars = 3 * STAGES + 5;
+    static constexpr int kSmem = 1024 + kData + kNumBars * 8 + 16;
+    static constexpr int kChain = 8;  // K blocks of 32 values
+    static constexpr int kTmemCols = 3 * BN <= 64 ? 64 : (3 * BN <= 128 ? 128 : (3 * BN <= 256 ? 256 : 512));
+    static_assert(kSmem <= 227 * 1024, "shared memory over the per-CTA limit");
+};
+
+// v = h + l + a rest below 2^-22 |v|, by integer rounding (the conversion instruction runs at a sixteenth of the rate: 279 us where this takes 140 for
+// 2048^3).  Not for what rounds to infinity, infinities and NaN.
+__device__ __forceinline__ void split_tf32(uint32_t v, uint32_t& h, uint32_t& l) {
+    h = (v + 0x1000u) & 0xffffe000u;
+    l = (__float_as_uint(__uint_as_float(v) - __uint_as_float(h)) + 0x1000u) & 0xffffe000u;
+}
+__device__ __forceinline__ bool rounds_away(uint32_t v) {  // to infinity, or it is one or NaN
+    return !(fabsf(__uint_as_float(v)) < __uint_as_float(0x7f7ff000u));
+}
+__device__ __forceinline__ void split_tf32_special(uint32_t v, uint32_t& h, uint32_t& l) {
+    const uint32_t a = v & 0x7fffffffu;
+    if (a < 0x7f7ff000u) return;
+    h = a > 0x7f800000u ? 0x7fffffffu : v & 0xffffe000u;  // NaN; infinity, or cut off instead of rounded
+    l = a >= 0x7f800000u ? 0u : __float_as_uint(__uint_as_float(v) - __uint_as_float(h)) & 0xffffe000u;
+}
+
+template <int BN, int STAGES>
+__global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const TcArgs p, int split,
+                                                              int x_tiles) {
+    using Cfg = TileF32Config<BN, STAGES>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kData);
+    uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto ready = [&](int s) { return bar0 + 8u * (STAGES + s); };  // split into h and l
+    auto empty = [&](int s) { return bar0 + 8u * (2 * STAGES + s); };
+    auto cfull = [&](int b) { return bar0 + 8u * (3 * STAGES + b); };       // a chain is complete in its accumulator
+    auto cempty = [&](int b) { return bar0 + 8u * (3 * STAGES + 2 + b); };  // ... and has been drained
+    const uint32_t done = bar0 + 8u * (3 * STAGES + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full(s), 2);
+            mbar_init(ready(s), 16);  // one arrival per splitting warp
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(cfull(b), 1);
+            mbar_init(cempty(b), 16);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_ptr), Cfg::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_ptr;  // accumulators: two chains by turns, then the small products
+    pdl_launch_dependents();
+    pdl_dependency_wait();
+
+    const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+    const int tile = (int)blockIdx.x / split;
+    const int x0 = (tile % x_tiles) * BN, w0 = (tile / x_tiles) * 128;
+    const int kb0 = (int)((int64_t)p.k_blocks * rank / split), blocks = (int)((int64_t)p.k_blocks * (rank + 1) / split) - kb0;  // at least one
+    const int chains = (blocks + Cfg::kChain - 1) / Cfg::kChain;
+    float* sums = reinterpret_cast<float*>(smem);
+    bool got = false;
+
+    if (warp < 4) {
+        if (lane == 0 && (warp == 0 || warp == 2)) {
+            const bool is_w = warp == 0;
+            for (int kb = 0; kb < blocks; ++kb) {
+                const int s = kb % STAGES;
+                if (!mbar_wait(empty(s), ((uint32_t)(kb / STAGES) & 1u) ^ 1u, abort_flag, p.status, 61, 0, p.wait_limit_ns)) break;
+                uint8_t* st = smem + s * Cfg::kStage;
+                mbar_expect_tx(full(s), is_w ? Cfg::kTileW : Cfg::kTileX);
+                if (is_w) tma_load_2d(smem_u32(st), &tmW, full(s), (kb0 + kb) * 128, w0);
+                else tma_load_2d(smem_u32(st + Cfg::kTileW), &tmX, full(s), (kb0 + kb) * 128, x0);
+            }
+        } else if (lane == 0 && warp == 1) {
+            bool ok = true;
+            const uint32_t hi = kmajor_desc_hi<128>(), idesc = idesc_tf32() | idesc_extents(128, BN);
+            for (int kb = 0; kb < blocks; ++kb) {
+                const int s = kb % STAGES, c = kb / Cfg::kChain, in = kb % Cfg::kChain;
+                if (in == 0 && !mbar_wait(cempty(c & 1), ((uint32_t)(c >> 1) & 1u) ^ 1u, abort_flag, p.status, 62, 0, p.wait_limit_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (!mbar_wait(ready(s), (uint32_t)(kb / STAGES) & 1u, abort_flag, p.status, 63, 0, p.wait_limit_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t st = smem_u32(smem + s * Cfg::kStage);
+                const uint32_t ah = kmajor_desc_lo(st), bh = kmajor_desc_lo(st + Cfg::kTileW), al = kmajor_desc_lo(st + Cfg::kRaw), bl = kmajor_desc_lo(st + Cfg::kRaw + Cfg::kTileW);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    umma_tf32(tmem + (uint32_t)((c & 1) * BN), ah + 2u * k, bh + 2u * k, hi, idesc, in > 0 || k > 0 ? 1u : 0u);
+                    umma_tf32(tmem + 2u * BN, ah + 2u * k, bl + 2u * k, hi, idesc, kb > 0 || k > 0 ? 1u : 0u);
+                    umma_tf32(tmem + 2u * BN, al + 2u * k, bh + 2u * k, hi, idesc, 1u);
+                }
+                umma_commit(empty(s));
+                if (in == Cfg::kChain - 1 || kb == blocks - 1) umma_commit(cfull(c & 1));
+            }
+            if (ok) umma_commit(done);
+        }
+        __syncwarp();
+    } else {
+        // Warps 4-19: one of four per 32 TMEM lanes (rows of w), and up to four for the columns (rows of x), at least sixteen columns each.
+        const int e = warp - 4, f = (warp & 3) * 32 + lane, part = e >> 2, tid = (int)threadIdx.x - 128;
+        constexpr int kParts = BN >= 64 ? 4 : BN / 16, kCols = BN / kParts;
+        const bool mine = part < kParts;
+        const uint32_t column0 = (uint32_t)(part * kCols), lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + column0;
+        float acc[kCols] = {};
+        got = true;
+        // Adds columns of TMEM; `finite`: only to sums that are -- next to an infinity the small products are NaN (infinity times l = 0).
+        auto add = [&](uint32_t at, bool finite) {
+#pragma unroll
+            for (int c = 0; c < kCols / 16; ++c) {
+                uint32_t r[16];
+                tmem_ld_32x32b_x16(at + (uint32_t)(c * 16), r);
+                tmem_ld_wait16(r);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (!finite || fabsf(acc[c * 16 + j]) < INFINITY) acc[c * 16 + j] += __uint_as_float(r[j]);
+            }
+        };
+        auto drain = [&](int c) {  // chain c into the registers; false: gave up
+            if (!__all_sync(0xffffffffu, mbar_wait(cfull(c & 1), (uint32_t)(c >> 1) & 1u, abort_flag, p.status, 64, 32, p.wait_limit_ns))) return false;
+            tc_fence_after();
+            if (mine) add(lanes + (uint32_t)((c & 1) * BN), false);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(cempty(c & 1));
+            return true;
+        };
+        for (int kb = 0; kb < blocks && got; ++kb) {
+            const int s = kb % STAGES;
+            got = __all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(kb / STAGES) & 1u, abort_flag, p.status, 65, 0, p.wait_limit_ns));
+            if (!got) break;
+            uint4* raw = reinterpret_cast<uint4*>(smem + s * Cfg::kStage);
+            uint4* low = reinterpret_cast<uint4*>(smem + s * Cfg::kStage + Cfg::kRaw);
+#pragma unroll 4
+            for (int i = tid; i < Cfg::kRaw / 16; i += 512) {
+                const uint4 v = raw[i];
+                uint4 h, l;
+                split_tf32(v.x, h.x, l.x);
+                split_tf32(v.y, h.y, l.y);
+                split_tf32(v.z, h.z, l.z);
+                split_tf32(v.w, h.w, l.w);
+                if (rounds_away(v.x) || rounds_away(v.y) || rounds_away(v.z) || rounds_away(v.w)) {
+                    split_tf32_special(v.x, h.x, l.x);
+                    split_tf32_special(v.y, h.y, l.y);
+                    split_tf32_special(v.z, h.z, l.z);
+                    split_tf32_special(v.w, h.w, l.w);
+                }
+                raw[i] = h;
+                low[i] = l;
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ready(s));
+            // the chain before the one that ends here has long been multiplied
+            if (kb % Cfg::kChain == Cfg::kChain - 1 && kb / Cfg::kChain > 0) got = drain(kb / Cfg::kChain - 1);
+        }
+        // what is left: the chain before the last, if its last block did not end a chain, and the last
+        if (got && chains > 1 && blocks % Cfg::kChain != 0) got = drain(chains - 2);
+        if (got) got = drain(chains - 1);
+        if (got) got = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, p.status, 66, 32, p.wait_limit_ns));
+        tc_fence_after();
+        // Every stage has been read; the warps write the sums together or not at all.
+        got = bar_all(1, 512, got);
+        if (got && mine) {
+            add(lanes + 2u * BN, true);
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) sums[((int)column0 + c) * 128 + f] = acc[c];
+        }
+    }
+    tc_fence_before();
+    if (split > 1) cluster_sync_all();
+    else __syncthreads();
+    if (got) tile_epilogue<float, BN, 16>(p, sums, x0, w0, rank, split, warp - 4, lane);
+    __syncthreads();
+    if (*abort_flag) {
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (split > 1) cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::kTmemCols);
