@@ -123,18 +123,25 @@ int launch_tile(F* kernel, int bn, int threads, int smem, KernelState& st, const
     if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * size, q.O, op.ldw * size, 128)) != CHXQ_OK) return rc;
     if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * size, q.M, op.ldx * size, bn)) != CHXQ_OK) return rc;
     const int64_t x_tiles = (q.M + bn - 1) / bn, tiles = x_tiles * ((q.O + 127) / 128);
-    // How many CTAs share a tile: what gives the fewest K blocks one after the other, a wave of clusters costing about kWave of them beside its own (launch,
+    // How many CTAs share a tile.  16-bit kernels, of which an SM holds two: doubled as long as there are no more CTAs than that and each has a K block.  One
+    // B200, in us by CTAs per tile: [1, 8192] x [8192, 8192]^T (64 tiles) 37.8, 28.5 with two, 25.2 with four, 30.7 with eight; [32, 4096] x [4096,
+    // 4096]^T (32 tiles) 21.0, 13.6, 9.8, 9.2.
+    // fp32 kernels fill an SM: what gives the fewest K blocks one after the other, a wave of clusters costing about kWave of them beside its own (launch,
     // first loads, joining the sums).  Clusters that do not all fit at once are worth less than smaller ones that do: [256, 2048] x [1000, 2048]^T
-    // in fp32 has 16 tiles, of which the GPU holds 14 or so as clusters of eight, and takes 30 us that way and 15 as clusters of four.
+    // has 16 tiles, of which the GPU holds 15 as clusters of eight, and takes 30 us that way and 20 as clusters of four.
     constexpr int64_t kWave = 6;
     int split = 1;
-    int64_t best = INT64_MAX;
-    for (int c = 1; c <= 8 && c <= args.k_blocks; ++c) {
-        const int64_t slots = cluster_slots(kernel, c, threads, smem, st, dev);
-        const int64_t cost = (tiles + slots - 1) / slots * ((args.k_blocks + c - 1) / c + kWave);
-        if (cost < best) {
-            best = cost;
-            split = c;
+    if (size == 2) {
+        while (split < 8 && tiles * split * 2 <= 2 * tc::sm_count() && split * 2 <= args.k_blocks) split *= 2;
+    } else {
+        int64_t best = INT64_MAX;
+        for (int c = 1; c <= 8 && c <= args.k_blocks; ++c) {
+            const int64_t slots = cluster_slots(kernel, c, threads, smem, st, dev);
+            const int64_t cost = (tiles + slots - 1) / slots * ((args.k_blocks + c - 1) / c + kWave);
+            if (cost < best) {
+                best = cost;
+                split = c;
+            }
         }
     }
     if (tiles * split >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: too many tiles");
@@ -182,11 +189,22 @@ int launch_pair(const chxq_linear_params& q, const Operands& op, const lin::TcAr
 
 template <typename T>
 int launch_tc(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
-    const int64_t blocks = ((q.M + 255) / 256) * ((q.O + 255) / 256);
-    if (q.M > 128 && blocks >= tc::sm_count() / 4) return launch_pair<T>(q, op, args, s);
+    const int64_t tiles128 = ((q.M + 127) / 128) * ((q.O + 127) / 128);
+    if (q.M > 128) {
+        // Pairs or single tiles, in units of 0.01 us from one B200: a K block of a 256 x 256 block takes a pair 0.27 us and a launch 6 beside that; a K
+        // block of a 128 x 128 tile takes an SM 0.27 us, too, and 0.3 at least where its CTA is alone.  [512, 4096] x [4096, 4096]^T: 25.3 us in
+        // pairs, 22.5 in tiles; [1024, 4096] x [4096, 4096]^T: 27.0 and 35.7; [8192, 64] x [1024, 64]^T: 10.1 and 18.8.
+        const int64_t sms = tc::sm_count(), blocks = ((q.M + 255) / 256) * ((q.O + 255) / 256), kb = args.k_blocks;
+        const int64_t pairs = (blocks + sms / 2 - 1) / (sms / 2) * kb * 27 + 600;
+        const int64_t share = std::min<int64_t>(8, std::max<int64_t>(1, 2 * sms / tiles128));
+        const int64_t tiles = std::max(tiles128 * kb * 27 / sms, (kb + share - 1) / share * 30) + 500 + tiles128 / (2 * sms) * 300;
+        if (pairs <= tiles) return launch_pair<T>(q, op, args, s);
+    }
     if (q.M <= 16) return launch_tile_16<T, 16, 6>(q, op, args, s);
     if (q.M <= 32) return launch_tile_16<T, 32, 5>(q, op, args, s);
-    if (q.M <= 64) return launch_tile_16<T, 64, 4>(q, op, args, s);
+    // Narrow tiles also where wide ones are so few that eight CTAs each do not fill the SMs twice: [256, 2048] x [1000, 2048]^T 9.1 against 10.5 us, [128,
+    // 4096] x [4096, 4096]^T 12.2 against 13.7.
+    if (q.M <= 64 || tiles128 <= 32) return launch_tile_16<T, 64, 4>(q, op, args, s);
     return launch_tile_16<T, 128, 3>(q, op, args, s);
 }
 

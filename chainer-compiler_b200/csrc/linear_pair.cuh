@@ -201,8 +201,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(bs + 4 * j) = *reinterpret_cast<const float4*>(s_bias + b * 64 + h * 16 + 4 * j);
                     tmem_ld_wait16(r);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-                    epilogue_apply<16, true>(p.e, v, bs, res);
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) + bs[j];
+                    epilogue_apply<16, true>(p.e, v, res);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         *reinterpret_cast<uint4*>(out + staged_offset<128>(row, 2 * h + j)) =

@@ -28,66 +28,96 @@ struct TileConfig {
 
 // From the shares of a tile, [BN][128] sums in the shared memory of each CTA of the cluster, to the outputs of this CTA's rows of x: the shares added in
 // ascending order (the same bits on every run), then bias, activation and residual.  `warp`: this one of WARPS.
-template <typename T, int BN, int WARPS>
-__device__ __forceinline__ void tile_epilogue(const TcArgs& p, const float* sums, int x0, int w0, int rank, int split, int warp, int lane) {
+// VEC: four neighbouring values per lane and access; else rows of y off 16-byte boundaries, lanes 32 values apart.  A few rows at a time, so that their loads
+// are in flight together ([509, 1283] x [2999, 1283]^T with a residual: 46 us one by one).
+template <typename T, int BN, int WARPS, bool VEC>
+__device__ __forceinline__ void tile_epilogue_rows(const TcArgs& p, const float* sums, int x0, int w0, int rank, int split, int warp, int lane) {
     constexpr bool kFast = sizeof(T) == 2;
+    constexpr int kRows = BN * 8 / WARPS >= 128 ? 4 : (BN >= 64 ? 2 : 1);
     const int cols = (BN + split - 1) / split;  // rows of x of this CTA
-    const bool vec = p.vec != 0;
-    auto feature = [&](int j) { return vec ? 4 * lane + j : lane + 32 * j; };
+    const int c1 = min(min((rank + 1) * cols, BN), p.M - x0);
+    auto feature = [&](int j) { return w0 + (VEC ? 4 * lane + j : lane + 32 * j); };
+    bool in[4];
     float bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bias[j] = p.e.bias && w0 + feature(j) < p.O ? load_param({p.e.bias, p.e.bias_dtype}, w0 + feature(j)) : 0.f;
-    const uint32_t sums0 = smem_u32(sums);
-    for (int c = rank * cols + warp; c < (rank + 1) * cols && c < BN && x0 + c < p.M; c += WARPS) {
-        const int64_t m = x0 + c;
-        float v[4] = {}, res[4] = {};
-        if (vec) {
-            if (w0 + 4 * lane >= p.O) continue;
-            for (int s = 0; s < split; ++s) {
-                float4 q;
-                const uint32_t at = sums0 + (uint32_t)(c * 128 + 4 * lane) * 4u;
-                if (split > 1)
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w) : "r"(map_to_cta(at, s)));
-                else
-                    q = *reinterpret_cast<const float4*>(sums + c * 128 + 4 * lane);
-                v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
-            }
-            const T* pr = static_cast<const T*>(p.e.residual) + m * p.e.ldr + w0 + 4 * lane;
-            T* py = static_cast<T*>(p.e.y) + m * p.e.ldy + w0 + 4 * lane;
-            if constexpr (sizeof(T) == 4) {
-                if (p.e.residual) {
-                    const float4 q = *reinterpret_cast<const float4*>(pr);
-                    res[0] = q.x; res[1] = q.y; res[2] = q.z; res[3] = q.w;
-                }
-                epilogue_apply<4, kFast>(p.e, v, bias, res);
-                *reinterpret_cast<float4*>(py) = make_float4(v[0], v[1], v[2], v[3]);
-            } else {
-                if (p.e.residual) {
-                    const uint2 q = *reinterpret_cast<const uint2*>(pr);
-                    const float2 lo = unpack16<T>(q.x), hi = unpack16<T>(q.y);
-                    res[0] = lo.x; res[1] = lo.y; res[2] = hi.x; res[3] = hi.y;
-                }
-                epilogue_apply<4, kFast>(p.e, v, bias, res);
-                *reinterpret_cast<uint2*>(py) = make_uint2(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]));
-            }
-        } else {
+    for (int j = 0; j < 4; ++j) {
+        in[j] = feature(j) < p.O;
+        bias[j] = p.e.bias && in[j] ? load_param({p.e.bias, p.e.bias_dtype}, feature(j)) : 0.f;
+    }
+    const uint32_t mine = smem_u32(sums) + (VEC ? 16u : 4u) * (uint32_t)lane;
+    for (int c0 = rank * cols + warp; c0 < c1; c0 += WARPS * kRows) {
+        float v[kRows * 4], res[kRows * 4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int f = feature(j);
-                for (int s = 0; s < split; ++s) {
-                    float q;
-                    if (split > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q) : "r"(map_to_cta(sums0 + (uint32_t)(c * 128 + f) * 4u, s)));
-                    else q = sums[c * 128 + f];
-                    v[j] += q;
-                }
-                if (p.e.residual && w0 + f < p.O) res[j] = to_f32(static_cast<const T*>(p.e.residual)[m * p.e.ldr + w0 + f]);
-            }
-            epilogue_apply<4, kFast>(p.e, v, bias, res);
+        for (int i = 0; i < kRows * 4; ++i) v[i] = bias[i % 4];
+        auto row = [&](int k) { return c0 + k * WARPS; };
+        auto have = [&](int k) { return kRows == 1 || row(k) < c1; };  // (reading another row in its place would double the traffic between the CTAs)
+        if (p.e.residual) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (w0 + feature(j) < p.O) static_cast<T*>(p.e.y)[m * p.e.ldy + w0 + feature(j)] = from_f32<T>(v[j]);
+            for (int k = 0; k < kRows; ++k) {
+                if (!have(k)) break;
+                const T* pr = static_cast<const T*>(p.e.residual) + (int64_t)(x0 + row(k)) * p.e.ldr;
+                if constexpr (!VEC) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (in[j]) res[4 * k + j] = to_f32(pr[feature(j)]);
+                } else if (in[0]) {
+                    if constexpr (sizeof(T) == 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(pr + feature(0));
+                        res[4 * k] = q.x; res[4 * k + 1] = q.y; res[4 * k + 2] = q.z; res[4 * k + 3] = q.w;
+                    } else {
+                        const uint2 q = *reinterpret_cast<const uint2*>(pr + feature(0));
+                        const float2 lo = unpack16<T>(q.x), hi = unpack16<T>(q.y);
+                        res[4 * k] = lo.x; res[4 * k + 1] = lo.y; res[4 * k + 2] = hi.x; res[4 * k + 3] = hi.y;
+                    }
+                }
+            }
+        }
+        // four shares at a time, their loads in flight together
+        for (int s0 = 0; s0 < split; s0 += 4) {
+            float q[4][kRows * 4] = {};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                if (s0 + s >= split) break;
+                const uint32_t from = split > 1 ? map_to_cta(mine, s0 + s) : mine;
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    if (!have(k)) break;
+                    const uint32_t at = from + (uint32_t)(row(k) * 512);
+                    if constexpr (VEC)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(q[s][4 * k]), "=f"(q[s][4 * k + 1]), "=f"(q[s][4 * k + 2]), "=f"(q[s][4 * k + 3])
+                                     : "r"(at));
+                    else
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q[s][4 * k + j]) : "r"(at + 128u * j));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                if (s0 + s < split)
+#pragma unroll
+                    for (int i = 0; i < kRows * 4; ++i) v[i] += q[s][i];
+        }
+        epilogue_apply<kRows * 4, kFast>(p.e, v, res);
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            if (!have(k)) break;
+            T* py = static_cast<T*>(p.e.y) + (int64_t)(x0 + c0 + k * WARPS) * p.e.ldy;
+            if constexpr (!VEC) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (in[j]) py[feature(j)] = from_f32<T>(v[4 * k + j]);
+            } else if (in[0]) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(py + feature(0)) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                else *reinterpret_cast<uint2*>(py + feature(0)) = make_uint2(pack16<T>(v[4 * k], v[4 * k + 1]), pack16<T>(v[4 * k + 2], v[4 * k + 3]));
+            }
         }
     }
+}
+template <typename T, int BN, int WARPS>
+__device__ __forceinline__ void tile_epilogue(const TcArgs& p, const float* sums, int x0, int w0, int rank, int split, int warp, int lane) {
+    if (p.vec) tile_epilogue_rows<T, BN, WARPS, true>(p, sums, x0, w0, rank, split, warp, lane);
+    else tile_epilogue_rows<T, BN, WARPS, false>(p, sums, x0, w0, rank, split, warp, lane);
 }
 
 template <typename T, int BN, int STAGES>
