@@ -20,19 +20,66 @@ struct LinearEpilogue {
 
 // Gelu through erfc, which keeps its relative accuracy where 1 + erf cancels; the tanh form as z / (1 + exp(-2 u)), for the same reason.
 // Large negative z: exp overflows to infinity and the quotient is -0, as the limit is.
-// FAST: exponential and quotient by the approximate instructions, a few 2^-22 relative and 2^-24 |z| more from the scaled argument: a
-// thousandth of a 16-bit output's rounding.
-template <int ACT, bool FAST = false>
+template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if constexpr (ACT == CHXQ_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays NaN
     if constexpr (ACT == CHXQ_ACT_GELU) return 0.5f * z * erfcf(z * -0.70710678118654752f);
+    if constexpr (ACT == CHXQ_ACT_GELU_TANH) return z / (1.f + expf(-1.5957691216057308f * (z + 0.044715f * z * z * z)));
+    if constexpr (ACT == CHXQ_ACT_SWISH) return z / (1.f + expf(-z));
+    if constexpr (ACT == CHXQ_ACT_SIGMOID) return 1.f / (1.f + expf(-z));
     if constexpr (ACT == CHXQ_ACT_TANH) return tanhf(z);
-    if constexpr (ACT == CHXQ_ACT_GELU_TANH || ACT == CHXQ_ACT_SWISH || ACT == CHXQ_ACT_SIGMOID) {
-        const float u = ACT == CHXQ_ACT_GELU_TANH ? -1.5957691216057308f * (z + 0.044715f * z * z * z) : -z;
-        const float d = 1.f + (FAST ? __expf(u) : expf(u)), n = ACT == CHXQ_ACT_SIGMOID ? 1.f : z;
-        return FAST ? __fdividef(n, d) : n / d;
-    }
     return z;
+}
+
+__device__ __forceinline__ f32x2 ex2_x2(f32x2 a) {  // 2^a, good to 2^-22
+    const float2 f = split_x2(a);
+    float x, y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(f.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(f.y));
+    return make_x2(x, y);
+}
+__device__ __forceinline__ f32x2 rcp_x2(f32x2 a) {  // 1 / a, good to 2^-23
+    const float2 f = split_x2(a);
+    float x, y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(f.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(f.y));
+    return make_x2(x, y);
+}
+__device__ __forceinline__ f32x2 both(float v) {
+    return make_x2(v, v);
+}
+
+// Two values at a time for 16-bit outputs, with exponential and reciprocal by the approximate instructions: a few 2^-22 relative, a thousandth of the
+// output's rounding.
+// Gelu: erfc by the Chebyshev fit of Press et al., Numerical Recipes, 6.2 ("erfcc", fractional error below 1.2e-7 everywhere): for u >= 0
+// erfc(u) = t exp(P(t) - u^2), t = 1 / (1 + u / 2); here with P and u^2 times log2 e.  [4096, 1024] x [4096, 1024]^T with Gelu on one B200: 55 us with
+// CUDA's erfcf.
+template <int ACT>
+__device__ __forceinline__ f32x2 activate_fast(f32x2 z) {
+    constexpr float L = 1.4426950408889634f;
+    if constexpr (ACT == CHXQ_ACT_GELU) {
+        const f32x2 u = mul2(z & 0x7fffffff7fffffffull, both(0.70710678118654752f));
+        const f32x2 t = rcp_x2(fma2(u, both(0.5f), both(1.f)));
+        f32x2 p = fma2(t, both(0.17087277f * L), both(-0.82215223f * L));
+        p = fma2(t, p, both(1.48851587f * L));
+        p = fma2(t, p, both(-1.13520398f * L));
+        p = fma2(t, p, both(0.27886807f * L));
+        p = fma2(t, p, both(-0.18628806f * L));
+        p = fma2(t, p, both(0.09678418f * L));
+        p = fma2(t, p, both(0.37409196f * L));
+        p = fma2(t, p, both(1.00002368f * L));
+        p = fma2(t, p, both(-1.26551223f * L));
+        const f32x2 e = mul2(t, ex2_x2(fma2(mul2(u, both(-L)), u, p)));
+        const float2 zf = split_x2(z), ef = split_x2(e);
+        return mul2(mul2(z, both(0.5f)), make_x2(zf.x < 0.f ? ef.x : 2.f - ef.x, zf.y < 0.f ? ef.y : 2.f - ef.y));
+    } else if constexpr (ACT == CHXQ_ACT_GELU_TANH || ACT == CHXQ_ACT_SWISH || ACT == CHXQ_ACT_SIGMOID) {
+        const f32x2 u = ACT == CHXQ_ACT_GELU_TANH ? mul2(z, fma2(mul2(z, z), both(-1.5957691216057308f * 0.044715f * L), both(-1.5957691216057308f * L))) : mul2(z, both(-L));
+        const f32x2 r = rcp_x2(add2(ex2_x2(u), both(1.f)));
+        return ACT == CHXQ_ACT_SIGMOID ? r : mul2(z, r);
+    } else {
+        const float2 f = split_x2(z);
+        return make_x2(activate<ACT>(f.x), activate<ACT>(f.y));
+    }
 }
 
 // Calls f(integral constant) with the activation code as a compile-time value (uniform over the grid).
@@ -56,7 +103,21 @@ __device__ __forceinline__ void epilogue_apply(const LinearEpilogue& e, float (&
     const bool first = e.residual_first;
     with_activation(e.activation, [&](auto act) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = activate<decltype(act)::value, FAST>(v[j] + (first ? res[j] : 0.f)) + (first ? 0.f : res[j]);
+        for (int j = 0; j < N; j += 2) {
+            const f32x2 r = make_x2(res[j], res[j + 1]);
+            f32x2 z = make_x2(v[j], v[j + 1]);
+            if (first) z = add2(z, r);
+            if constexpr (FAST) {
+                z = activate_fast<decltype(act)::value>(z);
+            } else {
+                const float2 f = split_x2(z);
+                z = make_x2(activate<decltype(act)::value>(f.x), activate<decltype(act)::value>(f.y));
+            }
+            if (!first) z = add2(z, r);
+            const float2 f = split_x2(z);
+            v[j] = f.x;
+            v[j + 1] = f.y;
+        }
     });
 }
 

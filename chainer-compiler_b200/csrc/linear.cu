@@ -176,13 +176,15 @@ int launch_pair(const chxq_linear_params& q, const Operands& op, const lin::TcAr
     a.m_blocks = (int)mb;
     a.o_blocks = (int)ob;
     a.tma_out = rows16(q.y, q.ldy, q.M, 2);
-    alignas(64) CUtensorMap tmX, tmW, tmY;
+    a.tma_res = q.residual && rows16(q.residual, q.ldr, q.M, 2);
+    alignas(64) CUtensorMap tmX, tmW, tmY, tmR;
     if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * 2, q.M, op.ldx * 2, 128)) != CHXQ_OK) return rc;
     if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * 2, q.O, op.ldw * 2, 128)) != CHXQ_OK) return rc;
-    tmY = tmX;  // not used where the output is copied
+    tmY = tmR = tmX;  // not used where the output is copied, and where there is no such residual
     if (a.tma_out && (rc = tc::encode_rows_map(&tmY, q.y, q.O * 2, q.M, q.ldy * 2, 128)) != CHXQ_OK) return rc;
+    if (a.tma_res && (rc = tc::encode_rows_map(&tmR, q.residual, q.O * 2, q.M, q.ldr * 2, 128)) != CHXQ_OK) return rc;
     const int pairs = (int)std::min<int64_t>(mb * ob, tc::sm_count() / 2);
-    CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), lin::kPairThreads, Cfg::kSmem, s, tmX, tmW, tmY, a));
+    CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)(2 * pairs)), lin::kPairThreads, Cfg::kSmem, s, tmX, tmW, tmY, tmR, a));
     count_launch(1);
     return CHXQ_OK;
 }

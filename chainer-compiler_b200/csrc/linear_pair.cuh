@@ -6,7 +6,8 @@
 // A CTA (352 threads): warp 0 loads x, warp 1 owns the TMEM and (first CTA of the pair) issues the MMAs, warp 2 loads w, warps 3-10 run the
 // epilogue.  Accumulators are double-buffered in TMEM, so the epilogue of a block runs under the main loop of the next.  The epilogue warps form two
 // groups of four (one warp per 32 TMEM lanes); a group takes every other 64 columns of the block, builds them as one swizzled
-// [128 rows][128 bytes] tile in shared memory and sends it with one TMA store (rows of y on 16-byte boundaries) or copies it out row by row.
+// [128 rows][128 bytes] tile in shared memory and sends it with one TMA store (rows of y on 16-byte boundaries) or copies it out row by row.  The
+// residual comes through TMA into that tile, the first 64 columns' under the main loop, the next ones' from the L2, where they are prefetched to.
 // What crosses the pair is as in tc_kernel3.cuh; no load is multicast.  Waits are bounded as there.
 #pragma once
 
@@ -22,7 +23,7 @@ struct PairConfig {
     static constexpr int kOut = kPairStages * kStage;            // two staged output tiles, one per epilogue group
     static constexpr int kBias = kOut + 2 * kTile;               // [256] floats
     static constexpr int kBars = kBias + 256 * 4;
-    static constexpr int kNumBars = 2 * kPairStages + 4;
+    static constexpr int kNumBars = 2 * kPairStages + 6;
     static constexpr int kSmem = 1024 + kBars + kNumBars * 8 + 16;
     static_assert(kSmem <= 227 * 1024, "shared memory over the per-CTA limit");
 };
@@ -31,11 +32,13 @@ struct PairArgs {
     TcArgs t;
     int m_blocks, o_blocks;  // blocks of 256 rows of x and of w
     int tma_out;             // the output leaves through tmY
+    int tma_res;             // the residual comes through tmR
 };
 
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY, const PairArgs a) {
+linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
+                   const __grid_constant__ CUtensorMap tmR, const PairArgs a) {
     using Cfg = PairConfig;
     const TcArgs& p = a.t;
     constexpr int kStages = kPairStages;
@@ -50,6 +53,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
     auto tfull = [&](int b) { return bar0 + 8u * (2 * kStages + b); };
     auto tempty = [&](int b) { return bar0 + 8u * (2 * kStages + 2 + b); };
+    auto rfull = [&](int g) { return bar0 + 8u * (2 * kStages + 4 + g); };  // residual tile of an epilogue group
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
 
@@ -61,6 +65,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         for (int b = 0; b < 2; ++b) {
             mbar_init(tfull(b), 1);
             mbar_init(tempty(b), 16);  // first CTA only: eight epilogue warps of each CTA
+            mbar_init(rfull(b), 1);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -152,13 +157,28 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         const bool issuer = (e & 3) == 0 && lane == 0;
         uint8_t* out = smem + Cfg::kOut + group * Cfg::kTile;
         const uint32_t lead_tempty = map_to_cta(tempty(0), 0);
+        uint32_t rphase = 0;
+        // (the issuer) 64 columns of the residual into the group's tile, once the store before has read it
+        auto fetch_residual = [&](int col, int m0) {
+            tma_store_wait_read<0>();
+            mbar_expect_tx(rfull(group), Cfg::kTile);
+            tma_load_2d(smem_u32(out), &tmR, rfull(group), col * (int)sizeof(T), m0);
+        };
         int it = 0;
-        for (int item = first; item < items; item += pairs, ++it) {
+        bool going = true;
+        for (int item = first; item < items && going; item += pairs, ++it) {
             const int buf = it & 1;
             int mb, ob;
             coords(item, mb, ob);
             const int m0 = mb * 256 + (int)rank * 128, o0 = ob * 256;
             const int64_t m = m0 + row;
+            if (a.tma_res && issuer) {
+                fetch_residual(o0 + group * 64, m0);
+                if (o0 + (group + 2) * 64 < p.O)
+                    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(&tmR)), "r"((o0 + (group + 2) * 64) * (int)sizeof(T)),
+                             "r"(m0)
+                             : "memory");
+            }
             bar_sync(1, 256);  // the last block's bias has been read
             s_bias[tid] = p.e.bias && o0 + tid < p.O ? load_param({p.e.bias, p.e.bias_dtype}, o0 + tid) : 0.f;
             // the bias is in place, and the eight warps go on or give up together: a warp that left alone would leave the others at a barrier
@@ -169,46 +189,54 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 #pragma unroll 1
             for (int b = group; b < 4; b += 2) {
                 const int col = o0 + b * 64;
-                if (issuer) tma_store_wait_read<0>();
-                bar_sync(2 + group, 128);  // the staged tile is free
-#pragma unroll 1
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t r[16];
-                    tmem_ld_32x32b_x16(taddr + (uint32_t)(b * 64 + h * 16), r);
-                    float res[16] = {}, v[16], bs[16];
-                    const int c0 = col + h * 16;
-                    if (p.e.residual && m < p.M) {
-                        const T* src = static_cast<const T*>(p.e.residual) + m * p.e.ldr + c0;
-                        if (p.vec && c0 + 16 <= p.O) {
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                const uint4 q = reinterpret_cast<const uint4*>(src)[j];
-                                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float2 f = unpack16<T>(w[i]);
-                                    res[8 * j + 2 * i] = f.x;
-                                    res[8 * j + 2 * i + 1] = f.y;
-                                }
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                if (c0 + j < p.O) res[j] = to_f32(src[j]);
+                if (a.tma_res) {
+                    if (b != group && issuer) fetch_residual(col, m0);
+                    const bool here = mbar_wait(rfull(group), rphase, abort_flag, p.status, 55, 32, p.wait_limit_ns);
+                    rphase ^= 1u;
+                    going = bar_all(1, 256, here);  // the eight warps go on or give up together, as above
+                    if (!going) break;
+                } else {
+                    if (issuer) tma_store_wait_read<0>();
+                    bar_sync(2 + group, 128);  // the staged tile is free
+                    if (p.e.residual) {
+                        // rows off 16-byte boundaries: a warp copies its 32 rows, 64 values each
+                        const int r0 = (e & 3) * 32, n = min(32, p.M - m0 - r0);
+                        const T* src = static_cast<const T*>(p.e.residual) + (int64_t)(m0 + r0) * p.e.ldr + col + lane;
+                        const bool in0 = col + lane < p.O, in1 = col + lane + 32 < p.O;
+#pragma unroll 8
+                        for (int i = 0; i < n; ++i, src += p.e.ldr) {
+                            const T v0 = in0 ? src[0] : from_f32<T>(0.f), v1 = in1 ? src[32] : from_f32<T>(0.f);
+                            *reinterpret_cast<T*>(out + staged_offset<128>(r0 + i, lane >> 3) + (lane & 7) * 2) = v0;
+                            *reinterpret_cast<T*>(out + staged_offset<128>(r0 + i, (lane >> 3) + 4) + (lane & 7) * 2) = v1;
                         }
+                        __syncwarp();
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(bs + 4 * j) = *reinterpret_cast<const float4*>(s_bias + b * 64 + h * 16 + 4 * j);
-                    tmem_ld_wait16(r);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) + bs[j];
-                    epilogue_apply<16, true>(p.e, v, res);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        *reinterpret_cast<uint4*>(out + staged_offset<128>(row, 2 * h + j)) =
-                                make_uint4(pack16<T>(v[8 * j], v[8 * j + 1]), pack16<T>(v[8 * j + 2], v[8 * j + 3]), pack16<T>(v[8 * j + 4], v[8 * j + 5]),
-                                           pack16<T>(v[8 * j + 6], v[8 * j + 7]));
                 }
+                uint32_t r[2][32];
+                tmem_ld_32x32b_x32(taddr + (uint32_t)(b * 64), r[0]);
+                tmem_ld_32x32b_x32(taddr + (uint32_t)(b * 64 + 32), r[1]);
+                tmem_ld_wait32(r[0]);
+                tmem_ld_wait32(r[1]);
+                const bool before = p.e.residual_first, res = p.e.residual != nullptr;
+                with_activation(p.e.activation, [&](auto act) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        T* cell = reinterpret_cast<T*>(out + staged_offset<128>(row, j));
+                        Pack<T, 8> o;
+                        if (res) o.load(cell);  // (rows past M hold what was there: their outputs are not stored)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = 8 * j + 2 * i;
+                            f32x2 z = add2(make_x2(__uint_as_float(r[c / 32][c % 32]), __uint_as_float(r[c / 32][c % 32 + 1])),
+                                           *reinterpret_cast<const f32x2*>(s_bias + b * 64 + c));
+                            if (res && before) z = add2(z, o.pair(i));
+                            z = activate_fast<decltype(act)::value>(z);
+                            if (res && !before) z = add2(z, o.pair(i));
+                            o.set_pair(i, z);
+                        }
+                        o.store(cell);
+                    }
+                });
                 if (b + 2 >= 4) {  // this warp's last read of the accumulators
                     tc_fence_before();
                     __syncwarp();
@@ -223,16 +251,17 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     }
                 } else {
                     // rows off 16-byte boundaries: a warp copies its 32 rows, 64 values each
-                    for (int i = 0; i < 32; ++i) {
-                        const int rr = (e & 3) * 32 + i;
-                        if (m0 + rr >= p.M) break;
-                        T* dst = static_cast<T*>(p.e.y) + (int64_t)(m0 + rr) * p.e.ldy + col;
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int c = lane + 32 * j;
-                            if (col + c < p.O) dst[c] = *reinterpret_cast<const T*>(out + staged_offset<128>(rr, c >> 3) + (c & 7) * 2);
-                        }
+                    const int r0 = (e & 3) * 32, n = min(32, p.M - m0 - r0);
+                    T* dst = static_cast<T*>(p.e.y) + (int64_t)(m0 + r0) * p.e.ldy + col + lane;
+                    const bool in0 = col + lane < p.O, in1 = col + lane + 32 < p.O;
+#pragma unroll 8
+                    for (int i = 0; i < n; ++i, dst += p.e.ldy) {
+                        const T v0 = *reinterpret_cast<const T*>(out + staged_offset<128>(r0 + i, lane >> 3) + (lane & 7) * 2);
+                        const T v1 = *reinterpret_cast<const T*>(out + staged_offset<128>(r0 + i, (lane >> 3) + 4) + (lane & 7) * 2);
+                        if (in0) dst[0] = v0;
+                        if (in1) dst[32] = v1;
                     }
+                    if (a.tma_res) bar_sync(2 + group, 128);  // the next residual is fetched into the tile that was copied from
                 }
             }
         }
