@@ -15,9 +15,15 @@
 
 #include "float_ops.cuh"
 #include "pdl.cuh"
+#include "tc_kernel.cuh"  // barriers with bounded waits
 
 namespace chxq {
 namespace {
+
+// `bytes` (a multiple of sixteen, both addresses on 16-byte boundaries) to shared memory; the barrier counts them.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 
 __device__ __forceinline__ void group_barrier(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -56,6 +62,17 @@ struct Place {
                     if (has(i, j)) v.put(j, row[column(i) + j]);
         }
     }
+    // The same for a row that is not looked at yet: nothing here waits for the load, so a piece that the thread does not have is left as it is.
+    __device__ __forceinline__ void load_ahead(const T* row, int i, bool last_row, Pack<T, VEC>& v) const {
+        const bool tail = SHIFT && last_row && column(i) + VEC > D;
+        if (any(i) && !tail) v.load(row + column(i));
+        if (tail) {
+            v.zero();
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (has(i, j)) v.put(j, row[column(i) + j]);
+        }
+    }
     // Zeroes the values of piece i that are not the row's.
     __device__ __forceinline__ void mask(int i, f32x2 (&v)[VEC / 2]) const {
         if (full(i)) return;
@@ -65,8 +82,24 @@ struct Place {
             v[j] = make_x2(has(i, 2 * j) ? f.x : 0.f, has(i, 2 * j + 1) ? f.y : 0.f);
         }
     }
-    __device__ __forceinline__ f32x2 param(const FloatArray& a, int i, int j) const {  // columns 2 j, 2 j + 1 of piece i
-        return make_x2(a.p && has(i, 2 * j) ? load_param(a, column(i) + 2 * j) : 0.f, a.p && has(i, 2 * j + 1) ? load_param(a, column(i) + 2 * j + 1) : 0.f);
+    // The columns' values of a parameter array; zero outside the row.  (The loads of a whole piece are in flight together; asked for one by one, each behind
+    // its own test, they took longer than the rest of a small gradient.)
+    __device__ __forceinline__ void params(const FloatArray& a, f32x2 (&f)[NV][VEC / 2]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[VEC] = {};
+            if (any(i)) {
+                if (full(i)) {
+                    load_params_any<T, VEC>(a, column(i), v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (has(i, j)) v[j] = load_param(a, column(i) + j);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) f[i][j] = make_x2(v[2 * j], v[2 * j + 1]);
+        }
     }
     __device__ __forceinline__ void store(T* row, int i, const Pack<T, VEC>& o) const {
         if (full(i)) {
@@ -250,13 +283,19 @@ __global__ void __launch_bounds__(kThreads) layernorm_long_kernel(const T* __res
 
 // ---- gradient -------------------------------------------------------------------------------------------------------------
 
-// Floats of the columns' sums of a block: [2][D], and of each of its warps where a warp holds several groups; in whole 16-byte pieces.
+// Floats of the columns' sums of a block: [2][D], of each of its warps where those go their own ways (G <= 32); in whole 16-byte pieces.
 __host__ __device__ constexpr int grad_sum_floats(int D, int G, int threads) {
-    return (2 * D * (G < 32 ? threads / 32 : 1) + 3) / 4 * 4;
+    return (2 * D * (G <= 32 ? threads / 32 : 1) + 3) / 4 * 4;
 }
 
-// As the forward pass, with two rows of operands.  The columns' sums over the rows stay in registers, or in shared memory (SMEM, one group: rows too
-// long for the registers of 512 threads), and leave as one partial sum [2][D] per block.
+// First row and distance of the rows of a group.  With SHIFT the groups of a block start at the same place of a piece: gridDim.x is a multiple of VEC.
+template <bool SHIFT, int VEC>
+__device__ __forceinline__ int64_t first_row(int groups, int group) {
+    return SHIFT ? blockIdx.x % VEC + VEC * ((int64_t)(blockIdx.x / VEC) * groups + group) : (int64_t)blockIdx.x * groups + group;
+}
+
+// Short rows, in groups of up to a warp (SMEM = false): every warp goes its own way, no barrier.  And rows too long for the registers of 512 threads, one
+// group, with the columns' sums in shared memory (SMEM).  The next row is fetched into registers.  Sums leave as one partial sum [2][D] per block.
 template <typename T, int NV, bool SHIFT, bool SMEM>
 __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, FloatArray scale,
                                                              const float* __restrict__ mean, const float* __restrict__ inv, int64_t rows, int D, int G,
@@ -268,7 +307,7 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
     pdl_dependency_wait();
     const int groups = (int)blockDim.x / G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t step = (int64_t)gridDim.x * groups;
-    int64_t r = (int64_t)blockIdx.x * groups + (int)threadIdx.x / G;
+    int64_t r = first_row<SHIFT, VEC>(groups, (int)threadIdx.x / G);
     const Place<T, NV, SHIFT> at(G, D, r, ldx);
     const T *px = x + r * ldx, *pd = dy + r * lddy;
     T* po = dx + r * D;
@@ -278,22 +317,21 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
     if (r < rows) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            at.load(px, i, r == rows - 1, nx[i]);
-            at.load(pd, i, r == rows - 1, nd[i]);
+            at.load_ahead(px, i, r == rows - 1, nx[i]);
+            at.load_ahead(pd, i, r == rows - 1, nd[i]);
         }
         nm = mean[r];
         ns = inv[r];
     }
     f32x2 g[NV][VEC / 2];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) g[i][j] = at.param(scale, i, j);
+    at.params(scale, g);
     f32x2 ag[SMEM ? 1 : NV][VEC / 2] = {}, ab[SMEM ? 1 : NV][VEC / 2] = {};
     for (int i = threadIdx.x; i < grad_sum_floats(D, G, (int)blockDim.x); i += blockDim.x) sums[i] = 0.f;
     __syncthreads();
     const float rd = 1.f / (float)D;
-    int64_t lead = G < 32 ? (int64_t)blockIdx.x * groups + ((int)threadIdx.x & ~31) / G : r;  // as in the forward pass
+    // Groups below 32 threads share warps, whose shuffles they all take part in: such a warp goes on until its first group, which has the most rows, is
+    // done.
+    int64_t lead = G < 32 ? r - (int64_t)(lane / G) * (SHIFT ? VEC : 1) : r;
     for (int par = 0; lead < rows; lead += step, r += step, par ^= 1) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -307,8 +345,8 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
         if (r + step < rows) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                at.load(px, i, r + step == rows - 1, nx[i]);
-                at.load(pd, i, r + step == rows - 1, nd[i]);
+                at.load_ahead(px, i, r + step == rows - 1, nx[i]);
+                at.load_ahead(pd, i, r + step == rows - 1, nd[i]);
             }
             nm = mean[r + step];
             ns = inv[r + step];
@@ -382,32 +420,217 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
     }
     __syncthreads();
     if constexpr (!SMEM) {
-        // In ascending order: groups of whole warps one after the other; smaller ones within their warp, each warp into sums of its own, which are
-        // then added.
-        const int warps = (int)blockDim.x >> 5;
-        for (int k = 0; k < (G < 32 ? 32 / G : groups); ++k) {
-            float* to = sums + (G < 32 ? 2 * D * warp : 0);
-            if ((G < 32 ? lane / G : at.group) == k)
+        // the groups of a warp, which have the same columns, by shuffles; the warps each in a place of their own, and then in ascending order
+        for (int o = G; o < 32; o <<= 1)
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (at.has(i, j)) {
-                            const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
-                            to[at.column(i) + j] += j & 1 ? fg.y : fg.x;
-                            to[D + at.column(i) + j] += j & 1 ? fb.y : fb.x;
-                        }
-            if (G < 32) __syncwarp();
-            else __syncthreads();
-        }
-        if (G < 32) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < 2 * D; i += blockDim.x)
-                for (int w = 1; w < warps; ++w) sums[i] += sums[2 * D * w + i];
-        }
+                for (int j = 0; j < VEC / 2; ++j) {
+                    ag[i][j] = add2(ag[i][j], __shfl_down_sync(0xffffffffu, ag[i][j], o));
+                    ab[i][j] = add2(ab[i][j], __shfl_down_sync(0xffffffffu, ab[i][j], o));
+                }
+        if (lane < G)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (at.has(i, j)) {
+                        const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
+                        sums[2 * D * warp + at.column(i) + j] = j & 1 ? fg.y : fg.x;
+                        sums[2 * D * warp + D + at.column(i) + j] = j & 1 ? fb.y : fb.x;
+                    }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * D; i += blockDim.x)
+            for (int w = 1; w < (int)blockDim.x >> 5; ++w) sums[i] += sums[2 * D * w + i];
     }
     float* mine = part + 2 * (int64_t)blockIdx.x * D;
     for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) mine[i] = sums[i];
+}
+
+// Rows in between, the common ones.  A group of G threads, whole warps, takes two rows at a time.  They come through a ring in shared memory, a row of x and
+// one of dy per stage by one bulk copy each, as far ahead as there is room: with the next row in registers 32 KB are in flight per SM, a
+// third less than the latency of the memory asks for.  Two rows share the barrier and hide each other's latencies; the second pass reads shared
+// memory again instead of holding both rows.  The columns' sums stay in registers.
+// (A wait that expires raises the status word; the loop then runs on to its end over whatever is there, so that no barrier is missed.)
+constexpr int kMaxStages = 8;
+template <typename T, bool SHIFT>
+__global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, FloatArray scale,
+                                                                  const float* __restrict__ mean, const float* __restrict__ inv, int64_t rows, int D, int G, int stages,
+                                                                  int row_bytes, T* __restrict__ dx, float* __restrict__ part, int* status, uint64_t wait_limit_ns) {
+    constexpr int VEC = 16 / (int)sizeof(T), NV = 2;
+    extern __shared__ __align__(16) uint8_t ring[];  // [groups][stages][x, dy][row_bytes]; the block's sums [2][D] in the end
+    __shared__ float red[2][16][4];
+    __shared__ uint64_t bars[16 / 2 * kMaxStages];
+    __shared__ int abort_flag;
+    const int groups = (int)blockDim.x / G, group = (int)threadIdx.x / G, lane = threadIdx.x & 31;
+    auto bar = [&](int s) { return tc::smem_u32(&bars[group * kMaxStages + s]); };
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < groups * kMaxStages; ++i) tc::mbar_init(tc::smem_u32(&bars[i]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    pdl_dependency_wait();
+    const int64_t step = (int64_t)gridDim.x * groups, first = first_row<SHIFT, VEC>(groups, group);
+    const Place<T, NV, SHIFT> at(G, D, first, ldx);
+    const int n = first < rows ? (int)((rows - first + step - 1) / step) : 0;
+    uint8_t* mine = ring + (size_t)group * stages * 2 * row_bytes;
+    // (one thread) Row k of the group into its stage.  The last row's last piece may reach past the buffer: it is copied value by value.
+    auto fetch = [&](int k, int stage) {
+        const int64_t r = first + k * step;
+        uint8_t* st = mine + (size_t)stage * 2 * row_bytes;
+        int bytes = row_bytes;
+        if constexpr (SHIFT) {
+            const int used = at.shift + D;  // values from the first piece's start to the row's end
+            bytes = (used + VEC - 1) / VEC * 16;
+            if (r == rows - 1 && used % VEC != 0) {
+                bytes -= 16;
+                for (int c = bytes / (int)sizeof(T); c < used; ++c) {
+                    reinterpret_cast<T*>(st)[c] = x[r * ldx + c - at.shift];
+                    reinterpret_cast<T*>(st + row_bytes)[c] = dy[r * lddy + c - at.shift];
+                }
+            }
+        }
+        tc::mbar_expect_tx(bar(stage), 2u * (uint32_t)bytes);
+        if (bytes > 0) {
+            bulk_load(tc::smem_u32(st), x + r * ldx - at.shift, (uint32_t)bytes, bar(stage));
+            bulk_load(tc::smem_u32(st + row_bytes), dy + r * lddy - at.shift, (uint32_t)bytes, bar(stage));
+        }
+    };
+    if (at.t == 0)
+        for (int k = 0; k < stages && k < n; ++k) fetch(k, k);
+    f32x2 g[NV][VEC / 2], ag[NV][VEC / 2] = {}, ab[NV][VEC / 2] = {};
+    at.params(scale, g);
+    const float rd = 1.f / (float)D;
+    auto read = [&](int stage, int which, int i, f32x2 (&v)[VEC / 2]) {
+        Pack<T, VEC> q;
+        q.load(reinterpret_cast<const T*>(mine + (stage * 2 + which) * row_bytes) + (at.t + i * G) * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) v[j] = q.pair(j);
+    };
+    float m[2] = {}, is[2] = {}, nm[2] = {}, ns[2] = {};
+    auto stats = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (k + u < n) {
+                nm[u] = mean[first + (k + u) * step];
+                ns[u] = inv[first + (k + u) * step];
+            }
+    };
+    stats(0);
+    int stage[2] = {0, 1}, phase[2] = {0, 0}, old[2] = {0, 0};  // of the two rows, and the stages of the two before
+    for (int k = 0; k < n; k += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            m[u] = nm[u];
+            is[u] = ns[u];
+        }
+        stats(k + 2);
+        float s[4] = {};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (k + u >= n) break;
+            tc::mbar_wait(bar(stage[u]), (uint32_t)phase[u], &abort_flag, status, 71, 0, wait_limit_ns);
+            const f32x2 is2 = make_x2(is[u], is[u]), nm2 = make_x2(-m[u], -m[u]);
+            f32x2 a = 0ull, b = 0ull;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!at.any(i)) continue;
+                f32x2 d[VEC / 2], h[VEC / 2];
+                read(stage[u], 0, i, h);
+                read(stage[u], 1, i, d);
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) h[j] = mul2(add2(h[j], nm2), is2);
+                if constexpr (SHIFT) {
+                    at.mask(i, d);
+                    at.mask(i, h);
+                }
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) {
+                    const f32x2 gd = mul2(d[j], g[i][j]);
+                    a = add2(a, gd);
+                    b = fma2(gd, h[j], b);
+                    ag[i][j] = fma2(d[j], h[j], ag[i][j]);
+                    ab[i][j] = add2(ab[i][j], d[j]);
+                }
+            }
+            const float2 fa = split_x2(a), fb = split_x2(b);
+            s[2 * u] = fa.x + fa.y;
+            s[2 * u + 1] = fb.x + fb.y;
+        }
+        // the sums of both rows over the group
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
+        const int par = (k >> 1) & 1, warps = G >> 5;
+        if (lane == 0) *reinterpret_cast<float4*>(red[par][threadIdx.x >> 5]) = make_float4(s[0], s[1], s[2], s[3]);
+        group_barrier(1 + group, G);
+        // every thread has left the rows before these: theirs are the stages to refill
+        if (at.t == 0 && k >= 2)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (k - 2 + u + stages < n) fetch(k - 2 + u + stages, old[u]);
+        {
+            const float4 q = (lane & 15) < warps ? *reinterpret_cast<const float4*>(red[par][group * warps + (lane & 15)]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            s[0] = q.x; s[1] = q.y; s[2] = q.z; s[3] = q.w;
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (k + u >= n) break;
+            const f32x2 is2 = make_x2(is[u], is[u]), nm2 = make_x2(-m[u], -m[u]), na = make_x2(-s[2 * u] * rd, -s[2 * u] * rd), nb = make_x2(-s[2 * u + 1] * rd, -s[2 * u + 1] * rd);
+            T* out = dx + (first + (k + u) * step) * D;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!at.any(i)) continue;
+                f32x2 d[VEC / 2], h[VEC / 2];
+                read(stage[u], 0, i, h);
+                read(stage[u], 1, i, d);
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC / 2; ++j) o.set_pair(j, mul2(fma2(d[j], g[i][j], fma2(mul2(add2(h[j], nm2), is2), nb, na)), is2));
+                at.store(out, i, o);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            old[u] = stage[u];
+            stage[u] += 2;
+            if (stage[u] >= stages) {
+                stage[u] -= stages;
+                phase[u] ^= 1;
+            }
+        }
+    }
+    __syncthreads();
+    if (abort_flag) {  // copies in flight get the time to land
+        const uint64_t t0 = tc::global_timer_ns();
+        while (tc::global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    float* sums = reinterpret_cast<float*>(ring);  // the groups' sums in ascending order
+    for (int k = 0; k < groups; ++k) {
+        if (group == k)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (at.has(i, j)) {
+                        const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
+                        const int c = at.column(i) + j;
+                        sums[c] = (k ? sums[c] : 0.f) + (j & 1 ? fg.y : fg.x);
+                        sums[D + c] = (k ? sums[D + c] : 0.f) + (j & 1 ? fb.y : fb.x);
+                    }
+        __syncthreads();
+    }
+    float* to = part + 2 * (int64_t)blockIdx.x * D;
+    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) to[i] = sums[i];
 }
 
 // Rows that neither holds: dx with the row read twice, and the parameters' sums in a pass of their own.
@@ -449,23 +672,29 @@ __global__ void __launch_bounds__(kThreads) layernorm_dparam_long_kernel(const T
     part[(2 * (int64_t)blockIdx.y + 1) * D + i] = b;
 }
 
-// part [shares][2 D] -> the sum of the shares: 32 columns a block, eight threads per column that take every eighth share.
-__global__ void __launch_bounds__(kThreads) layernorm_join_kernel(const float* __restrict__ part, int shares, int64_t D, int dtype, void* dscale, void* dbias) {
-    __shared__ float acc[8][33];
+// part [shares][2 D] -> the sum of the shares: 32 columns a block, a warp for every 32nd share (at most five each, loaded together).
+constexpr int kMaxBlocks = 148;  // of the gradient: one per SM
+__global__ void __launch_bounds__(1024) layernorm_join_kernel(const float* __restrict__ part, int shares, int64_t D, int dtype, void* dscale, void* dbias) {
+    __shared__ float acc[32][33];
     pdl_launch_dependents();
     pdl_dependency_wait();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+    constexpr int kEach = (kMaxBlocks + 31) / 32;
+    float v[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) v[k] = i < 2 * D && w + 32 * k < shares ? part[(int64_t)(w + 32 * k) * 2 * D + i] : 0.f;
     float a = 0.f;
-    if (i < 2 * D)
-        for (int s = w; s < shares; s += 8) a += part[(int64_t)s * 2 * D + i];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) a += v[k];
     acc[w][lane] = a;
     __syncthreads();
-    if (w == 0 && i < 2 * D) {
-#pragma unroll
-        for (int k = 1; k < 8; ++k) a += acc[k][lane];
-        if (i < D) store_param(dscale, dtype, i, a);
-        else if (dbias) store_param(dbias, dtype, i - D, a);
+    // column w of the block: its 32 sums by a warp
+    a = warp_sum(acc[lane][w]);
+    const int64_t c = (int64_t)blockIdx.x * 32 + w;
+    if (lane == 0 && c < 2 * D) {
+        if (c < D) store_param(dscale, dtype, c, a);
+        else if (dbias) store_param(dbias, dtype, c - D, a);
     }
 }
 
@@ -476,7 +705,7 @@ struct Plan {
 
 // Groups for `pieces` pieces of a row, nv each to a thread, in blocks of about `threads` threads, `per_sm` of them on an SM.  G is a power of two
 // within a warp, and whole warps above.  Where a row starts at another place of a 16-byte piece than the one before (shift), the number of
-// groups is a multiple of vec.
+// blocks is a multiple of vec.
 Plan plan_rows(int64_t pieces, int nv, int64_t rows, int threads, int per_sm, bool shift, int vec) {
     Plan p;
     const int64_t t = (pieces + nv - 1) / nv;
@@ -487,11 +716,7 @@ Plan plan_rows(int64_t pieces, int nv, int64_t rows, int threads, int per_sm, bo
     p.groups = std::max(least, threads / p.G);
     while (p.groups > least && (int64_t)p.groups * 148 > 2 * rows) p.groups = std::max(least, p.groups / 2);  // few rows: on more SMs
     int64_t blocks = std::min<int64_t>((rows + p.groups - 1) / p.groups, (int64_t)148 * per_sm);
-    if (shift) {
-        int unit = vec;  // blocks a multiple of it, and so the groups of vec
-        while (unit > 1 && p.groups * (unit / 2) % vec == 0) unit /= 2;
-        blocks = blocks > unit ? blocks / unit * unit : unit;  // not more than fit the SMs at a time
-    }
+    if (shift) blocks = blocks > vec ? blocks / vec * vec : vec;  // not more than fit the SMs at a time
     p.blocks = (int)blocks;
     return p;
 }
@@ -514,8 +739,6 @@ int launch_rows(F* kernel, const Plan& p, size_t smem, cudaStream_t s, Args... a
     count_launch(1);
     return CHXQ_OK;
 }
-
-constexpr int kMaxBlocks = 148;  // of the gradient: one per SM
 
 }  // namespace
 }  // namespace chxq
@@ -602,6 +825,18 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
             if (same_places(bits, rows, ldx, D, VEC) && same_places(bits, rows, lddy, D, VEC) && pieces <= nv * 512 && D <= 16 * 1024) {
                 const Plan p = plan_rows(pieces, nv, rows, 512, 1, shift, VEC);
                 shares = p.blocks;
+                if (nv == 2 && p.G > 32) {
+                    const int row_bytes = (int)pieces * 16;
+                    const int room = 220 * 1024, stages = std::min(kMaxStages, room / (p.groups * 2 * row_bytes));  // 32 KB a row and group at most: six
+                    const size_t smem = std::max((size_t)stages * p.groups * 2 * row_bytes, (size_t)2 * D * sizeof(float));
+                    int* status = device_status_ptr();
+                    if (!status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
+                    auto go = [&](auto* kernel) {
+                        return launch_rows(kernel, p, smem, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D, p.G, stages, row_bytes, static_cast<T*>(dx), part, status,
+                                           (uint64_t)tc::wait_limit_ns_value());
+                    };
+                    return shift ? go(layernorm_grad_ring_kernel<T, true>) : go(layernorm_grad_ring_kernel<T, false>);
+                }
                 auto go = [&](auto* kernel) {
                     return launch_rows(kernel, p, (size_t)grad_sum_floats((int)D, p.G, p.G * p.groups) * 4, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D, p.G,
                                        static_cast<T*>(dx), part);
@@ -619,7 +854,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
         });
         if (rc2 != CHXQ_OK) return rc2;
     }
-    CHXQ_CUDA(launch_pdl(layernorm_join_kernel, dim3((unsigned)((2 * D + 31) / 32)), kThreads, 0, s, static_cast<const float*>(part), shares, D, (int)affine_dtype, dscale,
+    CHXQ_CUDA(launch_pdl(layernorm_join_kernel, dim3((unsigned)((2 * D + 31) / 32)), 1024, 0, s, static_cast<const float*>(part), shares, D, (int)affine_dtype, dscale,
                          dbias));
     count_launch(1);
     return CHXQ_OK;
