@@ -126,8 +126,15 @@ struct Pack {
         return __half2float(*reinterpret_cast<const __half*>(&h));
     }
     __device__ __forceinline__ f32x2 pair(int i) const {  // values 2 i and 2 i + 1
-        if constexpr (sizeof(T) == 4) return make_x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-        else return make_x2(get(2 * i), get(2 * i + 1));
+        if constexpr (sizeof(T) == 4) {
+            return make_x2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const uint32_t v = w[i];
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+            return make_x2(f.x, f.y);
+        } else {
+            return make_x2(get(2 * i), get(2 * i + 1));
+        }
     }
     __device__ __forceinline__ void set_pair(int i, f32x2 v) {
         const float2 f = split_x2(v);

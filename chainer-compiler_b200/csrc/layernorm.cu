@@ -36,12 +36,15 @@ struct Place {
     static constexpr int VEC = 16 / (int)sizeof(T);
     int G, group, t;  // threads per group (a power of two up to 32, or a multiple of 32), this thread's group and place in it
     int shift;        // columns of the row before in the group's first piece
-    int D;
+    int D;            // end of this block's columns: the row's, or the end of its share of the pieces
+    int p0;           // first piece of that share
 
-    __device__ __forceinline__ Place(int G_, int D_, int64_t row0, int64_t ld) : G(G_), group((int)threadIdx.x / G_), t((int)threadIdx.x % G_), D(D_) {
+    __device__ __forceinline__ Place(int G_, int D_, int64_t row0, int64_t ld, int p0_ = 0, int share = 0)
+        : G(G_), group((int)threadIdx.x / G_), t((int)threadIdx.x % G_), D(D_), p0(p0_) {
         shift = SHIFT ? (int)((row0 * ld) & (VEC - 1)) : 0;
+        if (share) D = min(D, (p0 + share) * VEC - shift);
     }
-    __device__ __forceinline__ int column(int i) const { return (t + i * G) * VEC - shift; }  // the first of piece i; negative ones belong to the row before
+    __device__ __forceinline__ int column(int i) const { return (p0 + t + i * G) * VEC - shift; }  // the first of piece i; negative ones belong to the row before
     __device__ __forceinline__ bool any(int i) const { return FULL || column(i) < D; }
     __device__ __forceinline__ bool full(int i) const { return !SHIFT || (column(i) >= 0 && column(i) + VEC <= D); }
     __device__ __forceinline__ bool has(int i, int j) const { return (unsigned)(column(i) + j) < (unsigned)D; }
@@ -112,10 +115,9 @@ struct Place {
     }
 };
 
-// Sum over a group of G threads, the same for all of them; at most sixteen warps.  red: [2][warps of the block] per value, used by turns (par), so
-// that one barrier is enough.
+// Sums over a group of G <= 32 threads, the same for all of them.
 template <int N>
-__device__ __forceinline__ void group_sum(float (&v)[N], int G, int group, float (*red)[32][N], int par) {
+__device__ __forceinline__ void group_sum(float (&v)[N], int G) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -123,20 +125,6 @@ __device__ __forceinline__ void group_sum(float (&v)[N], int G, int group, float
             const float q = __shfl_xor_sync(0xffffffffu, v[k], o);
             if (o < G) v[k] += q;
         }
-    if (G <= 32) return;
-    const int lane = threadIdx.x & 31, warps = G >> 5;
-    if (lane == 0)
-#pragma unroll
-        for (int k = 0; k < N; ++k) red[par][threadIdx.x >> 5][k] = v[k];
-    group_barrier(1 + group, G);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = lane < warps ? red[par][group * warps + lane][k] : 0.f;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = __shfl_sync(0xffffffffu, v[k], 0);
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------
@@ -283,31 +271,30 @@ __global__ void __launch_bounds__(kThreads) layernorm_long_kernel(const T* __res
 
 // ---- gradient -------------------------------------------------------------------------------------------------------------
 
-// Floats of the columns' sums of a block: [2][D], of each of its warps where those go their own ways (G <= 32); in whole 16-byte pieces.
-__host__ __device__ constexpr int grad_sum_floats(int D, int G, int threads) {
-    return (2 * D * (G <= 32 ? threads / 32 : 1) + 3) / 4 * 4;
+// Floats of the columns' sums of a block: [2][D] of each of its warps.
+__host__ __device__ constexpr int grad_sum_floats(int D, int threads) {
+    return 2 * D * (threads / 32);
 }
 
 // First row and distance of the rows of a group.  With SHIFT the groups of a block start at the same place of a piece: gridDim.x is a multiple of VEC.
 template <bool SHIFT, int VEC>
-__device__ __forceinline__ int64_t first_row(int groups, int group) {
-    return SHIFT ? blockIdx.x % VEC + VEC * ((int64_t)(blockIdx.x / VEC) * groups + group) : (int64_t)blockIdx.x * groups + group;
+__device__ __forceinline__ int64_t first_row(int block, int groups, int group) {
+    return SHIFT ? block % VEC + VEC * ((int64_t)(block / VEC) * groups + group) : (int64_t)block * groups + group;
 }
 
-// Short rows, in groups of up to a warp (SMEM = false): every warp goes its own way, no barrier.  And rows too long for the registers of 512 threads, one
-// group, with the columns' sums in shared memory (SMEM).  The next row is fetched into registers.  Sums leave as one partial sum [2][D] per block.
-template <typename T, int NV, bool SHIFT, bool SMEM>
+// Short rows, in groups of up to a warp: every warp goes its own way, no barrier.  The next row is fetched into registers.  The columns' sums leave as one
+// partial sum [2][D] per block.
+template <typename T, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, FloatArray scale,
                                                              const float* __restrict__ mean, const float* __restrict__ inv, int64_t rows, int D, int G,
                                                              T* __restrict__ dx, float* __restrict__ part) {
     constexpr int VEC = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) float sums[];
-    __shared__ float red[2][32][2];
     pdl_launch_dependents();
     pdl_dependency_wait();
     const int groups = (int)blockDim.x / G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t step = (int64_t)gridDim.x * groups;
-    int64_t r = first_row<SHIFT, VEC>(groups, (int)threadIdx.x / G);
+    int64_t r = first_row<SHIFT, VEC>((int)blockIdx.x, groups, (int)threadIdx.x / G);
     const Place<T, NV, SHIFT> at(G, D, r, ldx);
     const T *px = x + r * ldx, *pd = dy + r * lddy;
     T* po = dx + r * D;
@@ -325,14 +312,14 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
     }
     f32x2 g[NV][VEC / 2];
     at.params(scale, g);
-    f32x2 ag[SMEM ? 1 : NV][VEC / 2] = {}, ab[SMEM ? 1 : NV][VEC / 2] = {};
-    for (int i = threadIdx.x; i < grad_sum_floats(D, G, (int)blockDim.x); i += blockDim.x) sums[i] = 0.f;
+    f32x2 ag[NV][VEC / 2] = {}, ab[NV][VEC / 2] = {};
+    for (int i = threadIdx.x; i < grad_sum_floats(D, (int)blockDim.x); i += blockDim.x) sums[i] = 0.f;
     __syncthreads();
     const float rd = 1.f / (float)D;
     // Groups below 32 threads share warps, whose shuffles they all take part in: such a warp goes on until its first group, which has the most rows, is
     // done.
-    int64_t lead = G < 32 ? r - (int64_t)(lane / G) * (SHIFT ? VEC : 1) : r;
-    for (int par = 0; lead < rows; lead += step, r += step, par ^= 1) {
+    int64_t lead = r - (int64_t)(lane / G) * (SHIFT ? VEC : 1);
+    for (; lead < rows; lead += step, r += step) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             vx[i] = nx[i];
@@ -372,40 +359,14 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
                     const f32x2 gd = mul2(d[j], g[i][j]);
                     a = add2(a, gd);
                     b = fma2(gd, h[j], b);
-                    if constexpr (!SMEM) {
-                        ag[i][j] = fma2(d[j], h[j], ag[i][j]);
-                        ab[i][j] = add2(ab[i][j], d[j]);
-                    }
-                }
-                if constexpr (SMEM) {
-                    float *pg = sums + at.column(i), *pb = pg + D;
-#pragma unroll
-                    for (int j = 0; j < VEC / 2; j += 2) {
-                        if constexpr (!SHIFT) {  // whole 16-byte pieces, of columns and of sums
-                            ulonglong2 *qg = reinterpret_cast<ulonglong2*>(pg + 2 * j), *qb = reinterpret_cast<ulonglong2*>(pb + 2 * j), vg = *qg, vb = *qb;
-                            vg.x = fma2(d[j], h[j], vg.x);
-                            vg.y = fma2(d[j + 1], h[j + 1], vg.y);
-                            vb.x = add2(vb.x, d[j]);
-                            vb.y = add2(vb.y, d[j + 1]);
-                            *qg = vg;
-                            *qb = vb;
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (at.has(i, 2 * j + k)) {
-                                    const float2 fd = split_x2(d[j + k / 2]), fh = split_x2(h[j + k / 2]);
-                                    const float e = k & 1 ? fd.y : fd.x;
-                                    pg[2 * j + k] = fmaf(e, k & 1 ? fh.y : fh.x, pg[2 * j + k]);
-                                    pb[2 * j + k] += e;
-                                }
-                        }
-                    }
+                    ag[i][j] = fma2(d[j], h[j], ag[i][j]);
+                    ab[i][j] = add2(ab[i][j], d[j]);
                 }
             }
         }
         const float2 fa = split_x2(a), fb = split_x2(b);
         float s[2] = {fa.x + fa.y, fb.x + fb.y};
-        group_sum<2>(s, G, at.group, red, par);
+        group_sum<2>(s, G);
         const f32x2 na = make_x2(-s[0] * rd, -s[0] * rd), nb = make_x2(-s[1] * rd, -s[1] * rd);
         if (r < rows)
 #pragma unroll
@@ -419,47 +380,50 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
         po += so;
     }
     __syncthreads();
-    if constexpr (!SMEM) {
-        // the groups of a warp, which have the same columns, by shuffles; the warps each in a place of their own, and then in ascending order
-        for (int o = G; o < 32; o <<= 1)
+    // the groups of a warp, which have the same columns, by shuffles; the warps each in a place of their own, and then in ascending order
+    for (int o = G; o < 32; o <<= 1)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC / 2; ++j) {
-                    ag[i][j] = add2(ag[i][j], __shfl_down_sync(0xffffffffu, ag[i][j], o));
-                    ab[i][j] = add2(ab[i][j], __shfl_down_sync(0xffffffffu, ab[i][j], o));
+            for (int j = 0; j < VEC / 2; ++j) {
+                ag[i][j] = add2(ag[i][j], __shfl_down_sync(0xffffffffu, ag[i][j], o));
+                ab[i][j] = add2(ab[i][j], __shfl_down_sync(0xffffffffu, ab[i][j], o));
+            }
+    if (lane < G)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (at.has(i, j)) {
+                    const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
+                    sums[2 * D * warp + at.column(i) + j] = j & 1 ? fg.y : fg.x;
+                    sums[2 * D * warp + D + at.column(i) + j] = j & 1 ? fb.y : fb.x;
                 }
-        if (lane < G)
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (at.has(i, j)) {
-                        const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
-                        sums[2 * D * warp + at.column(i) + j] = j & 1 ? fg.y : fg.x;
-                        sums[2 * D * warp + D + at.column(i) + j] = j & 1 ? fb.y : fb.x;
-                    }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 2 * D; i += blockDim.x)
-            for (int w = 1; w < (int)blockDim.x >> 5; ++w) sums[i] += sums[2 * D * w + i];
-    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x)
+        for (int w = 1; w < (int)blockDim.x >> 5; ++w) sums[i] += sums[2 * D * w + i];
     float* mine = part + 2 * (int64_t)blockIdx.x * D;
     for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) mine[i] = sums[i];
 }
 
-// Rows in between, the common ones.  A group of G threads, whole warps, takes two rows at a time.  They come through a ring in shared memory, a row of x and
-// one of dy per stage by one bulk copy each, as far ahead as there is room: with the next row in registers 32 KB are in flight per SM, a
-// third less than the latency of the memory asks for.  Two rows share the barrier and hide each other's latencies; the second pass reads shared
-// memory again instead of holding both rows.  The columns' sums stay in registers.
+// Rows in between, the common ones.  A group of G threads, whole warps, takes ROWS rows at a time: two, or one where the ring has no more than
+// three stages.  They come through a ring in shared memory, a row of x and one of dy per stage by one bulk copy each, as far ahead as there is
+// room: with the next row in registers 32 KB are in flight per SM, a third less than the latency of the memory asks for.  Two rows share the barrier
+// and hide each other's latencies; the second pass reads shared memory again instead of holding both rows.  The columns' sums stay in registers.
+// Rows too long for the registers of 512 threads: the CL blocks of a cluster take a share of the columns each (one group per block), and the rows'
+// sums meet across them; one block with its sums in shared memory took 153 us for [4096, 16384] bf16 and 280 for [4096, 12345].
 // (A wait that expires raises the status word; the loop then runs on to its end over whatever is there, so that no barrier is missed.)
+// [8192, 8192] bf16: 86 us, 73% of a copy's rate (the instructions of two passes over 16-bit values bound it); [16384, 4096] fp32 122 us, the
+// memory's; [8192, 8192] fp32 140 us (89%); [4096, 16384] bf16 102 us, [4096, 12345] bf16 103 us, [4096, 14001] fp32 137 us.
 constexpr int kMaxStages = 8;
-template <typename T, bool SHIFT>
+template <typename T, int NV, bool SHIFT, int CL, int ROWS>
 __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, FloatArray scale,
                                                                   const float* __restrict__ mean, const float* __restrict__ inv, int64_t rows, int D, int G, int stages,
                                                                   int row_bytes, T* __restrict__ dx, float* __restrict__ part, int* status, uint64_t wait_limit_ns) {
-    constexpr int VEC = 16 / (int)sizeof(T), NV = 2;
+    // (row_bytes: of a block's share of a row)
+    constexpr int VEC = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) uint8_t ring[];  // [groups][stages][x, dy][row_bytes]; the block's sums [2][D] in the end
-    __shared__ float red[2][16][4];
+    __shared__ __align__(16) float red[2][16 * CL][4];
     __shared__ uint64_t bars[16 / 2 * kMaxStages];
     __shared__ int abort_flag;
     const int groups = (int)blockDim.x / G, group = (int)threadIdx.x / G, lane = threadIdx.x & 31;
@@ -471,32 +435,34 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
+    if constexpr (CL > 1) tc::cluster_sync_all();  // the blocks write into one another's shared memory: all have started
     pdl_launch_dependents();
     pdl_dependency_wait();
-    const int64_t step = (int64_t)gridDim.x * groups, first = first_row<SHIFT, VEC>(groups, group);
-    const Place<T, NV, SHIFT> at(G, D, first, ldx);
+    const int rank = CL > 1 ? (int)tc::cluster_ctarank() : 0, share = row_bytes / 16;
+    const int64_t step = (int64_t)(gridDim.x / CL) * groups, first = first_row<SHIFT, VEC>((int)blockIdx.x / CL, groups, group);
+    const Place<T, NV, SHIFT> at(G, D, first, ldx, rank * share, CL > 1 ? share : 0);
+    const int64_t start = rank * share * VEC - at.shift;  // the first piece's column
     const int n = first < rows ? (int)((rows - first + step - 1) / step) : 0;
     uint8_t* mine = ring + (size_t)group * stages * 2 * row_bytes;
     // (one thread) Row k of the group into its stage.  The last row's last piece may reach past the buffer: it is copied value by value.
     auto fetch = [&](int k, int stage) {
         const int64_t r = first + k * step;
         uint8_t* st = mine + (size_t)stage * 2 * row_bytes;
-        int bytes = row_bytes;
+        const int used = max(0, at.D - (int)start);  // values from the first piece's start to the end of the share
+        int bytes = (used + VEC - 1) / VEC * 16;
         if constexpr (SHIFT) {
-            const int used = at.shift + D;  // values from the first piece's start to the row's end
-            bytes = (used + VEC - 1) / VEC * 16;
             if (r == rows - 1 && used % VEC != 0) {
                 bytes -= 16;
                 for (int c = bytes / (int)sizeof(T); c < used; ++c) {
-                    reinterpret_cast<T*>(st)[c] = x[r * ldx + c - at.shift];
-                    reinterpret_cast<T*>(st + row_bytes)[c] = dy[r * lddy + c - at.shift];
+                    reinterpret_cast<T*>(st)[c] = x[r * ldx + start + c];
+                    reinterpret_cast<T*>(st + row_bytes)[c] = dy[r * lddy + start + c];
                 }
             }
         }
         tc::mbar_expect_tx(bar(stage), 2u * (uint32_t)bytes);
         if (bytes > 0) {
-            bulk_load(tc::smem_u32(st), x + r * ldx - at.shift, (uint32_t)bytes, bar(stage));
-            bulk_load(tc::smem_u32(st + row_bytes), dy + r * lddy - at.shift, (uint32_t)bytes, bar(stage));
+            bulk_load(tc::smem_u32(st), x + r * ldx + start, (uint32_t)bytes, bar(stage));
+            bulk_load(tc::smem_u32(st + row_bytes), dy + r * lddy + start, (uint32_t)bytes, bar(stage));
         }
     };
     if (at.t == 0)
@@ -510,27 +476,29 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j) v[j] = q.pair(j);
     };
-    float m[2] = {}, is[2] = {}, nm[2] = {}, ns[2] = {};
+    float m[ROWS] = {}, is[ROWS] = {}, nm[ROWS] = {}, ns[ROWS] = {};
     auto stats = [&](int k) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < ROWS; ++u)
             if (k + u < n) {
                 nm[u] = mean[first + (k + u) * step];
                 ns[u] = inv[first + (k + u) * step];
             }
     };
     stats(0);
-    int stage[2] = {0, 1}, phase[2] = {0, 0}, old[2] = {0, 0};  // of the two rows, and the stages of the two before
-    for (int k = 0; k < n; k += 2) {
+    int stage[ROWS], phase[ROWS] = {}, old[ROWS] = {};  // of these rows, and the stages of those before
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < ROWS; ++u) stage[u] = u;
+    for (int k = 0; k < n; k += ROWS) {
+#pragma unroll
+        for (int u = 0; u < ROWS; ++u) {
             m[u] = nm[u];
             is[u] = ns[u];
         }
-        stats(k + 2);
+        stats(k + ROWS);
         float s[4] = {};
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROWS; ++u) {
             if (k + u >= n) break;
             tc::mbar_wait(bar(stage[u]), (uint32_t)phase[u], &abort_flag, status, 71, 0, wait_limit_ns);
             const f32x2 is2 = make_x2(is[u], is[u]), nm2 = make_x2(-m[u], -m[u]);
@@ -564,25 +532,35 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
-        const int par = (k >> 1) & 1, warps = G >> 5;
-        if (lane == 0) *reinterpret_cast<float4*>(red[par][threadIdx.x >> 5]) = make_float4(s[0], s[1], s[2], s[3]);
-        group_barrier(1 + group, G);
+            for (int q = 0; q < 2 * ROWS; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
+        const int par = (k / ROWS) & 1, warps = G >> 5;
+        if constexpr (CL == 1) {
+            if (lane == 0) *reinterpret_cast<float4*>(red[par][threadIdx.x >> 5]) = make_float4(s[0], s[1], s[2], s[3]);
+            group_barrier(1 + group, G);
+        } else {
+            if (lane < CL)  // to every block of the cluster
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(tc::map_to_cta(tc::smem_u32(red[par][rank * warps + (int)(threadIdx.x >> 5)]), (uint32_t)lane)),
+                             "f"(s[0]), "f"(s[1]), "f"(s[2]), "f"(s[3])
+                             : "memory");
+            __syncwarp();
+            tc::cluster_sync_all();
+        }
         // every thread has left the rows before these: theirs are the stages to refill
-        if (at.t == 0 && k >= 2)
+        if (at.t == 0 && k >= ROWS)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (k - 2 + u + stages < n) fetch(k - 2 + u + stages, old[u]);
-        {
-            const float4 q = (lane & 15) < warps ? *reinterpret_cast<const float4*>(red[par][group * warps + (lane & 15)]) : make_float4(0.f, 0.f, 0.f, 0.f);
-            s[0] = q.x; s[1] = q.y; s[2] = q.z; s[3] = q.w;
+            for (int u = 0; u < ROWS; ++u)
+                if (k - ROWS + u + stages < n) fetch(k - ROWS + u + stages, old[u]);
+        s[0] = s[1] = s[2] = s[3] = 0.f;
+        for (int e = lane & 15; e < CL * warps; e += 16) {
+            const float4 q = *reinterpret_cast<const float4*>(red[par][(CL == 1 ? group * warps : 0) + e]);
+            s[0] += q.x; s[1] += q.y; s[2] += q.z; s[3] += q.w;
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
+            for (int q = 0; q < 2 * ROWS; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROWS; ++u) {
             if (k + u >= n) break;
             const f32x2 is2 = make_x2(is[u], is[u]), nm2 = make_x2(-m[u], -m[u]), na = make_x2(-s[2 * u] * rd, -s[2 * u] * rd), nb = make_x2(-s[2 * u + 1] * rd, -s[2 * u + 1] * rd);
             T* out = dx + (first + (k + u) * step) * D;
@@ -599,9 +577,9 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
             }
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROWS; ++u) {
             old[u] = stage[u];
-            stage[u] += 2;
+            stage[u] += ROWS;
             if (stage[u] >= stages) {
                 stage[u] -= stages;
                 phase[u] ^= 1;
@@ -614,23 +592,39 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
         while (tc::global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
         __syncthreads();
     }
-    float* sums = reinterpret_cast<float*>(ring);  // the groups' sums in ascending order
+    if constexpr (CL > 1) tc::cluster_sync_all();  // the others may still be writing into this block's `red`
+    // the groups' sums in ascending order, in the order of the pieces
+    float* sums = reinterpret_cast<float*>(ring);
+    const int cols = share * VEC;
     for (int k = 0; k < groups; ++k) {
         if (group == k)
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                if (!at.any(i)) continue;
+                // (whole pieces: what a thread has of the rows beside its own is zero)
+                ulonglong2 *pg = reinterpret_cast<ulonglong2*>(sums + (at.t + i * G) * VEC), *pb = reinterpret_cast<ulonglong2*>(sums + cols + (at.t + i * G) * VEC);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (at.has(i, j)) {
-                        const float2 fg = split_x2(ag[i][j / 2]), fb = split_x2(ab[i][j / 2]);
-                        const int c = at.column(i) + j;
-                        sums[c] = (k ? sums[c] : 0.f) + (j & 1 ? fg.y : fg.x);
-                        sums[D + c] = (k ? sums[D + c] : 0.f) + (j & 1 ? fb.y : fb.x);
+                for (int j = 0; j < VEC / 4; ++j) {
+                    ulonglong2 vg = make_ulonglong2(ag[i][2 * j], ag[i][2 * j + 1]), vb = make_ulonglong2(ab[i][2 * j], ab[i][2 * j + 1]);
+                    if (k) {
+                        const ulonglong2 og = pg[j], ob = pb[j];
+                        vg = make_ulonglong2(add2(og.x, vg.x), add2(og.y, vg.y));
+                        vb = make_ulonglong2(add2(ob.x, vb.x), add2(ob.y, vb.y));
                     }
+                    pg[j] = vg;
+                    pb[j] = vb;
+                }
+            }
         __syncthreads();
     }
-    float* to = part + 2 * (int64_t)blockIdx.x * D;
-    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) to[i] = sums[i];
+    float* to = part + 2 * (int64_t)(blockIdx.x / CL) * D;
+    for (int i = threadIdx.x; i < cols; i += blockDim.x) {
+        const int c = (int)start + i;
+        if (c >= 0 && c < at.D) {
+            to[c] = sums[i];
+            to[D + c] = sums[cols + i];
+        }
+    }
 }
 
 // Rows that neither holds: dx with the row read twice, and the parameters' sums in a pass of their own.
@@ -672,29 +666,33 @@ __global__ void __launch_bounds__(kThreads) layernorm_dparam_long_kernel(const T
     part[(2 * (int64_t)blockIdx.y + 1) * D + i] = b;
 }
 
-// part [shares][2 D] -> the sum of the shares: 32 columns a block, a warp for every 32nd share (at most five each, loaded together).
+// part [shares][2 D] -> the sum of the shares: 32 columns a block; warps that take every eighth share (up to 40 shares) or every 32nd, at most five each,
+// loaded together.
 constexpr int kMaxBlocks = 148;  // of the gradient: one per SM
 __global__ void __launch_bounds__(1024) layernorm_join_kernel(const float* __restrict__ part, int shares, int64_t D, int dtype, void* dscale, void* dbias) {
     __shared__ float acc[32][33];
     pdl_launch_dependents();
     pdl_dependency_wait();
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     const int64_t i = (int64_t)blockIdx.x * 32 + lane;
-    constexpr int kEach = (kMaxBlocks + 31) / 32;
+    constexpr int kEach = 5;
+    static_assert(kEach * 32 >= kMaxBlocks, "shares per warp");
     float v[kEach];
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) v[k] = i < 2 * D && w + 32 * k < shares ? part[(int64_t)(w + 32 * k) * 2 * D + i] : 0.f;
+    for (int k = 0; k < kEach; ++k) v[k] = i < 2 * D && w + warps * k < shares ? part[(int64_t)(w + warps * k) * 2 * D + i] : 0.f;
     float a = 0.f;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) a += v[k];
     acc[w][lane] = a;
     __syncthreads();
-    // column w of the block: its 32 sums by a warp
-    a = warp_sum(acc[lane][w]);
-    const int64_t c = (int64_t)blockIdx.x * 32 + w;
-    if (lane == 0 && c < 2 * D) {
-        if (c < D) store_param(dscale, dtype, c, a);
-        else if (dbias) store_param(dbias, dtype, c - D, a);
+    if (w == 0 && i < 2 * D) {
+        a = 0.f;
+        for (int k = 0; k < warps; k += 8) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) a += acc[k + q][lane];
+        }
+        if (i < D) store_param(dscale, dtype, i, a);
+        else if (dbias) store_param(dbias, dtype, i - D, a);
     }
 }
 
@@ -821,29 +819,50 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
             const uintptr_t bits = reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dx);
             const bool shift = D % VEC != 0;
             const int64_t pieces = pieces_of(D, VEC, shift);
-            const int nv = pieces <= 2 * 512 ? 2 : (pieces <= 4 * 512 ? 4 : 8);  // from four on with the columns' sums in shared memory
-            if (same_places(bits, rows, ldx, D, VEC) && same_places(bits, rows, lddy, D, VEC) && pieces <= nv * 512 && D <= 16 * 1024) {
-                const Plan p = plan_rows(pieces, nv, rows, 512, 1, shift, VEC);
+            // Columns of a block in the registers of 512 threads, two pieces each, or four of fp32 (sixteen values at most); longer rows shared by the blocks of a
+            // cluster.
+            const int nv = VEC == 4 && pieces > 1024 ? 4 : 2, cl = pieces <= nv * 512 ? 1 : (pieces <= nv * 1024 ? 2 : 4);
+            if (same_places(bits, rows, ldx, D, VEC) && same_places(bits, rows, lddy, D, VEC) && pieces <= (VEC == 4 ? 4 : 2) * (VEC == 4 ? 1024 : 2048)) {
+                const int64_t share = (pieces + cl - 1) / cl;
+                Plan p = plan_rows(share, nv, rows, 512, 1, shift, VEC);
+                if (cl > 1) {
+                    const int64_t most = cl == 2 ? 74 : 32;  // clusters that are resident at once (of four: 33)
+                    p.blocks = (int)std::min<int64_t>(std::max<int64_t>(rows, 1), most);
+                    if (shift) p.blocks = p.blocks > VEC ? p.blocks / VEC * VEC : VEC;
+                }
                 shares = p.blocks;
-                if (nv == 2 && p.G > 32) {
-                    const int row_bytes = (int)pieces * 16;
-                    const int room = 220 * 1024, stages = std::min(kMaxStages, room / (p.groups * 2 * row_bytes));  // 32 KB a row and group at most: six
-                    const size_t smem = std::max((size_t)stages * p.groups * 2 * row_bytes, (size_t)2 * D * sizeof(float));
+                if (p.G > 32) {
+                    const int row_bytes = (int)share * 16;
+                    const int room = 220 * 1024, stages = std::min(kMaxStages, room / (p.groups * 2 * row_bytes));
+                    // the groups' sums are not laid out by row but by piece: also those of pieces that hold no column
+                    const size_t smem = std::max((size_t)stages * p.groups * 2 * row_bytes, (size_t)2 * share * VEC * sizeof(float));
                     int* status = device_status_ptr();
                     if (!status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
                     auto go = [&](auto* kernel) {
-                        return launch_rows(kernel, p, smem, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D, p.G, stages, row_bytes, static_cast<T*>(dx), part, status,
-                                           (uint64_t)tc::wait_limit_ns_value());
+                        CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                        CHXQ_CUDA(launch_pdl_cluster(cl, kernel, dim3((unsigned)(p.blocks * cl)), p.G * p.groups, smem, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D,
+                                                     p.G, stages, row_bytes, static_cast<T*>(dx), part, status, (uint64_t)tc::wait_limit_ns_value()));
+                        count_launch(1);
+                        return CHXQ_OK;
                     };
-                    return shift ? go(layernorm_grad_ring_kernel<T, true>) : go(layernorm_grad_ring_kernel<T, false>);
+                    constexpr int kMost = 16 / VEC;  // pieces of a thread
+                    // Two rows at a time need four stages: those of the rows before are refilled while these are worked on.  A share of up to 16 KB (nv == 2)
+                    // leaves six or more, one of up to 32 KB three or more.
+                    const bool one = stages < 4;
+                    if (nv == 2 && cl == 1) return shift ? go(layernorm_grad_ring_kernel<T, 2, true, 1, 2>) : go(layernorm_grad_ring_kernel<T, 2, false, 1, 2>);
+                    if constexpr (VEC == 4) {
+                        if (one && cl == 1) return shift ? go(layernorm_grad_ring_kernel<T, 4, true, 1, 1>) : go(layernorm_grad_ring_kernel<T, 4, false, 1, 1>);
+                        if (one) return shift ? go(layernorm_grad_ring_kernel<T, 4, true, 2, 1>) : go(layernorm_grad_ring_kernel<T, 4, false, 2, 1>);
+                        if (cl == 1) return shift ? go(layernorm_grad_ring_kernel<T, 4, true, 1, 2>) : go(layernorm_grad_ring_kernel<T, 4, false, 1, 2>);
+                    }
+                    if (cl == 2) return shift ? go(layernorm_grad_ring_kernel<T, kMost, true, 2, 2>) : go(layernorm_grad_ring_kernel<T, kMost, false, 2, 2>);
+                    if constexpr (VEC == 8) return shift ? go(layernorm_grad_ring_kernel<T, 2, true, 4, 2>) : go(layernorm_grad_ring_kernel<T, 2, false, 4, 2>);
                 }
                 auto go = [&](auto* kernel) {
-                    return launch_rows(kernel, p, (size_t)grad_sum_floats((int)D, p.G, p.G * p.groups) * 4, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D, p.G,
+                    return launch_rows(kernel, p, (size_t)grad_sum_floats((int)D, p.G * p.groups) * 4, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D, p.G,
                                        static_cast<T*>(dx), part);
                 };
-                if (nv == 2) return shift ? go(layernorm_grad_kernel<T, 2, true, false>) : go(layernorm_grad_kernel<T, 2, false, false>);
-                if (nv == 4) return shift ? go(layernorm_grad_kernel<T, 4, true, true>) : go(layernorm_grad_kernel<T, 4, false, true>);
-                if constexpr (VEC == 4) return shift ? go(layernorm_grad_kernel<T, 8, true, true>) : go(layernorm_grad_kernel<T, 8, false, true>);
+                return shift ? go(layernorm_grad_kernel<T, 2, true>) : go(layernorm_grad_kernel<T, 2, false>);
             }
             layernorm_dx_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kThreads, 0, s>>>(g, lddy, v, ldx, sc, mean, inv_std_dev, rows, D, static_cast<T*>(dx));
             CHXQ_LAUNCH_CHECK();
@@ -854,7 +873,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
         });
         if (rc2 != CHXQ_OK) return rc2;
     }
-    CHXQ_CUDA(launch_pdl(layernorm_join_kernel, dim3((unsigned)((2 * D + 31) / 32)), 1024, 0, s, static_cast<const float*>(part), shares, D, (int)affine_dtype, dscale,
+    CHXQ_CUDA(launch_pdl(layernorm_join_kernel, dim3((unsigned)((2 * D + 31) / 32)), shares <= 40 ? 256 : 1024, 0, s, static_cast<const float*>(part), shares, D, (int)affine_dtype, dscale,
                          dbias));
     count_launch(1);
     return CHXQ_OK;

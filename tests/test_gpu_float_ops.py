@@ -244,6 +244,14 @@ def test_layernorm_grad_extents(ops, dev, dtype, rows, d):
     _check_grad(ops, dev, rows, d, dtype, torch.float32, pitch=3)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,d", [(20001, 520), (6001, 1030), (3001, 4999), (2405, 8192), (1501, 12001), (1203, 16384), (803, 28000)])
+def test_layernorm_grad_of_many_rows(ops, dev, dtype, rows, d):
+    """More rows than a block holds at once, several times over: what holds the rows is filled again and again, and no wait runs out."""
+    _check_grad(ops, dev, rows, d, dtype, dtype)
+    ops.device_status()
+
+
 def test_layernorm_grad_against_differences(ops, dev):
     g = torch.Generator(device=dev).manual_seed(11)
     x, dy = torch.randn((6, 40), device=dev, generator=g), torch.randn((6, 40), device=dev, generator=g)
