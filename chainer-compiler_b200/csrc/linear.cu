@@ -1,14 +1,15 @@
 // Linear with bias, activation and residual in its epilogue: y = act(x w^T + b) + r, or act(x w^T + b + r); bf16, fp16 and fp32 operands,
 // sums in 32 bits, one rounding at the end.
 //
-// Two kernels: CTA pairs with 256 x 256 blocks (linear_pair.cuh) for large 16-bit products, and clusters that share a tile's K (linear_tile.cuh) for
-// few rows of x, for products in between and for fp32.
+// Three kernels: CTA pairs with 256 x 256 blocks (linear_pair.cuh) for large 16-bit products, clusters that share a tile's K (linear_tile.cuh) for
+// few rows of x, for products in between and for fp32, and threads side by side along K for a few rows of fp32 (linear_rows.cuh).
 #include <algorithm>
 #include <atomic>
 
 #include "epilogue_float.cuh"
 #include "float_ops.cuh"
 #include "linear_pair.cuh"
+#include "linear_rows.cuh"
 #include "linear_tile.cuh"
 
 namespace chxq {
@@ -218,6 +219,28 @@ int launch_tc<float>(const chxq_linear_params& q, const Operands& op, const lin:
     return launch_tile_32<128, 3>(q, op, args, s);
 }
 
+// A few rows of fp32.  No alignment is asked for: rows off 16-byte boundaries are read value by value ([1, 2147] x [2999, 2147]^T: 8 us, and 27 with copies in
+// front of tiles).
+template <int MR>
+int launch_rows(const chxq_linear_params& q, const LinearEpilogue& e, cudaStream_t s) {
+    constexpr int R = 4;
+    const bool vec = rows16(q.x, q.ldx, q.M, 4) && rows16(q.w, q.ldw, q.O, 4);
+    const int64_t blocks = (q.O + R - 1) / R, pieces = vec ? q.K / 4 : q.K;
+    const int threads = (int)std::min<int64_t>(blocks <= tc::sm_count() ? 512 : 256, std::max<int64_t>(32, (pieces + 31) / 32 * 32));
+    auto* kernel = vec ? lin::linear_rows_kernel<MR, R, 4, MR <= 2 ? 4 : (MR == 4 ? 2 : 1)> : lin::linear_rows_kernel<MR, R, 1, MR <= 2 ? 8 : 4>;
+    CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)blocks, (unsigned)((q.M + MR - 1) / MR)), threads, 0, s, static_cast<const float*>(q.x), q.ldx, static_cast<const float*>(q.w), q.ldw, (int)q.M, (int)q.O,
+                         (int)q.K, e));
+    count_launch(1);
+    return CHXQ_OK;
+}
+
+// Up to eight rows, one block for all of them; up to sixteen, two blocks for eight each, where the blocks run in two waves (two are on an SM at once):
+// [16, 2048] x [1000, 2048]^T 6.5 us against 11.6 in tiles, [16, 1024] x [4096, 1024]^T 15.2 against 11.7.
+bool few_rows(const chxq_linear_params& q) {
+    if (q.dtype != CHXQ_FLOAT32 || q.M > lin::kRowsMost) return false;
+    return q.M <= 8 || (q.O + 3) / 4 * 2 <= 4 * tc::sm_count();
+}
+
 }  // namespace
 }  // namespace chxq
 
@@ -238,7 +261,7 @@ static int check_linear(const chxq_linear_params* p) {
 }
 
 extern "C" size_t chxq_linear_workspace(const chxq_linear_params* p) {
-    if (!p || !is_float_type(p->dtype) || p->K <= 0 || p->M <= 0 || p->O <= 0) return 0;
+    if (!p || !is_float_type(p->dtype) || p->K <= 0 || p->M <= 0 || p->O <= 0 || few_rows(*p)) return 0;
     const int size = float_size(p->dtype);
     size_t n = 0;
     if (!rows16(p->x, p->ldx, p->M, size)) n += align256((size_t)(p->M * pitch16(p->K, size)) * size);
@@ -261,6 +284,11 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
             CHXQ_LAUNCH_CHECK();
             return CHXQ_OK;
         });
+    if (few_rows(*p)) {
+        if (p->M == 1) return launch_rows<1>(*p, e, s);
+        if (p->M == 2) return launch_rows<2>(*p, e, s);
+        return p->M <= 4 ? launch_rows<4>(*p, e, s) : launch_rows<8>(*p, e, s);
+    }
     const int size = float_size(p->dtype);
     Operands op = {p->x, p->ldx, p->w, p->ldw};
     if (need) {

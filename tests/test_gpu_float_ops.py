@@ -86,6 +86,12 @@ def test_linear_rows_of_wider_buffers(ops, dev, dtype, pitch, m):
     _check_linear(ops, dev, m, 320, 264, dtype, "Swish", "last", pitch=pitch)
 
 
+@pytest.mark.parametrize("m", list(range(1, 10)) + [16])
+@pytest.mark.parametrize("k,o,pitch", [(4100, 5, 0), (1023, 131, 0), (70, 2050, 1), (3, 64, 4), (6948, 26, 0), (2047, 700, 5)])
+def test_linear_few_rows_of_fp32(ops, dev, m, k, o, pitch):
+    _check_linear(ops, dev, m, k, o, torch.float32, "Tanh", "first" if m % 2 else "last", pitch=pitch)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_offset_addresses_and_other_strides(ops, dev, dtype):
     """Operands that start off a 16-byte boundary, a transposed weight, rows that overlap (an expanded one), a batch of leading dimensions."""
