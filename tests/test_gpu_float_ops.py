@@ -434,7 +434,7 @@ def _check_logprobs_grad(ops, dev, x, tok, seed=0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,v", [(1, 1), (3, 7), (256, 1000), (5, 1001), (2, 50001), (1, 131072), (700, 129)])
+@pytest.mark.parametrize("rows,v", [(1, 1), (3, 7), (256, 1000), (5, 1001), (2, 50001), (1, 131072), (700, 129), (2003, 303), (77, 509), (77, 510), (9, 1017), (9, 1018), (41, 13)])
 def test_token_logprobs_grad_extents(ops, dev, dtype, rows, v):
     g = torch.Generator(device=dev).manual_seed(rows * 3 + v)
     x = (torch.randn((rows, v), device=dev, generator=g) * 3).to(dtype)
