@@ -10,11 +10,14 @@ read on the host once per call as the reference's GetScalar does, runtime/chxvm_
 without a bias input and every MatMul first becomes the dynamic IntegerOps sequence of compiler/quantize.cc:142-281 --
 ReduceMin / ReduceMax -> scale, zero point -> QuantizeLinear -> ConvInteger / MatMulInteger -> Cast -> Mul.  With
 `--fuse_operations --use_nvrtc` the float Add / Sub / Mul / Tanh / Sigmoid / Exp glue is grouped as the reference groups it
-(compiler/fusion_elementwise.cc:10-40) and every group runs as one generated kernel (ElementWiseNvrtc).  The remaining float
-glue (Relu, MaxPool, Reshape, Cast, BatchNormalization, ...) is outside the quantized hot path and runs as torch tensor
-expressions on the same device.  A float Conv / MatMul / Gemm has no kernel here and is refused, unless
-`--float_ops_via_torch` asks for the torch expression (useful to check a test directory's expected outputs; not a code path of
-the product).
+(compiler/fusion_elementwise.cc:10-40) and every group runs as one generated kernel (ElementWiseNvrtc).  A float MatMul or Gemm with constant weights
+runs as Linear, with the bias, activation and residual Add behind it in its epilogue (fuse_linear); LayerNormalization,
+SoftmaxCrossEntropyLoss (without class weights) and this package's own nodes LayerNormalizationGrad (dy, x, scale, mean,
+inv_std_dev), TokenLogProbs (logits, tokens) and TokenLogProbsGrad (dlogprob, dentropy, logits, tokens, log_sum_exp, entropy)
+run on the operators of those names.  The remaining float glue (Relu, MaxPool, Reshape, Cast, BatchNormalization, ...) is
+outside the hot path and runs as torch tensor expressions on the same device.  A float Conv, or a MatMul of two computed
+operands, has no kernel here and is refused, unless `--float_ops_via_torch` asks for the torch expression (useful to check a
+test directory's expected outputs; not a code path of the product; every float MatMul and Gemm is one then).
 
 Compile passes, in the reference's order (compiler/passes.cc:121-128): constant folding of Reshape over initializers,
 Quantize, then MergeConvBN (compiler/merge.cc:142-215) over the Conv nodes that are still float.  `--fold_bn_first` swaps the
@@ -25,8 +28,10 @@ On a statically quantized graph two peepholes run unless `--no_peephole` is give
 QuantizeLinear (a residual join) becomes one uint8 kernel, and a QLinearConv whose only reader is such a join takes it into its
 epilogue; both keep every output bit.  Convolutions with constant weights are packed once and run on the tensor-core kernels
 over channels_last activations.  Options of this build beyond the reference's: `--fold_scales` (one fp32 multiplier per output
-channel in the requantization instead of a multiply and a divide; up to one output step of difference) and `--cuda_graph`
-(with -I > 1 a program without device-to-host reads is captured after the first iteration and replayed).
+channel in the requantization instead of a multiply and a divide; up to one output step of difference), `--cuda_graph`
+(with -I > 1 a program without device-to-host reads is captured after the first iteration and replayed) and `--top K` (the K
+most probable entries along the last dimension of every float output, with their log probabilities and that of the expected
+output's largest entry; also in the report).
 
 Flags kept from the reference: positional or --test DIR / --onnx FILE, -d/--device, -I/--iterations, --rtol, --atol,
 --equal_nan, --no_check_values, --always_show_diff, --check_nans, --check_infs, --dump_outputs_dir (one
@@ -127,11 +132,12 @@ def merge_conv_bn(nodes, consts, graph_outputs=(), only=None):
     return [n for n in out if id(n) not in dropped]
 
 
-def compile_model(model, quantize=False, per_channel=True, asymmetric_input_types=False, fold_bn_first=False, fuse=False, peephole=True):
+def compile_model(model, quantize=False, per_channel=True, asymmetric_input_types=False, fold_bn_first=False, fuse=False, peephole=True,
+                  float_linear=True):
     """ONNX graph -> Program.  quantize: the reference's `--quantize` (dynamic, IntegerOps; weights uint8 unless
     asymmetric_input_types, which makes them int8: compiler/quantize.cc:392-400).  fuse: group elementwise float nodes into
     ElementWiseNvrtc instructions (`--fuse_operations --use_nvrtc`).  peephole: True = fuse_quantized_add, then fuse_conv_residual;
-    "join" = the first only; False = neither."""
+    "join" = the first only; False = neither.  float_linear: float products with constant weights become Linear (fuse_linear)."""
     nodes, consts = _fold_constants(model)
 
     def quantizable(n):
@@ -205,6 +211,8 @@ def compile_model(model, quantize=False, per_channel=True, asymmetric_input_type
         program = fuse_quantized_add(program)
         if peephole != "join":
             program = fuse_stem(fuse_conv_residual(program))
+    if float_linear:
+        program = fuse_linear(program, epilogue=bool(peephole))
     if fuse:
         program = fuse_elementwise(program)
     return program
@@ -350,6 +358,101 @@ def fuse_stem(program):
     return Program(_topological(new, set(program.constants) | set(program.inputs)), program.constants, program.inputs, program.outputs)
 
 
+def fuse_linear(program, epilogue=True):
+    """A float product with constant weights becomes one Linear instruction: MatMul [..., K] x [K, O], and Gemm without transA,
+    alpha and beta (a float32 Gemm with transB is left as it is: the executor runs it as Linear already).  With `epilogue` it
+    takes what follows it as single-use values: an Add of a constant [O] or [1, O] (the bias), then Relu, Tanh, Sigmoid, Gelu or x *
+    Sigmoid(x) and an Add of a computed value (the residual), in either order.  The weights are laid out as [O, K] once, here.
+    Inputs: x, weights, bias or "", residual or "".  The replaced nodes stay in `members`, for the export."""
+    insts = program.insts
+    users = {}
+    for k, i in enumerate(insts):
+        for v in i.inputs:
+            users.setdefault(v, []).append(k)
+    consts = program.constants
+    floats = (np.float32, np.float16)
+
+    def readers(v, n):
+        u = users.get(v, [])
+        return u if len(u) == n and v not in program.outputs and not taken.intersection(u) else []
+
+    def vector(name, o, dtype):
+        c = consts.get(name)
+        return c is not None and np.asarray(c).dtype == dtype and np.asarray(c).size == o and np.asarray(c).shape[-1:] == (o,)
+
+    replaced, taken, added, dropped = {}, set(), {}, set()
+    for k, i in enumerate(insts):
+        if k in taken or i.op not in ("MatMul", "Gemm") or len(i.inputs) < 2 or i.inputs[0] in consts or i.inputs[1] not in consts:
+            continue
+        w = np.asarray(consts[i.inputs[1]])
+        if w.ndim != 2 or w.dtype not in floats:
+            continue
+        trans = i.op == "Gemm" and bool(i.attrs.get("transB", 0))
+        bias = ""
+        if i.op == "Gemm":
+            if i.attrs.get("transA", 0) or i.attrs.get("alpha", 1.0) != 1.0 or i.attrs.get("beta", 1.0) != 1.0 or (trans and w.dtype == np.float32):
+                continue
+            if len(i.inputs) > 2 and i.inputs[2] != "":
+                bias = i.inputs[2]
+                if not vector(bias, w.shape[0 if trans else 1], w.dtype):
+                    continue
+        o = w.shape[0 if trans else 1]
+        chain, v = [k], i.outputs[0]
+        if epilogue and not bias:
+            u = readers(v, 1)
+            if u and insts[u[0]].op == "Add":
+                other = [t for t in insts[u[0]].inputs if t != v]
+                if len(other) == 1 and vector(other[0], o, w.dtype):
+                    bias, chain, v = other[0], chain + u, insts[u[0]].outputs[0]
+
+        def take_activation(v):
+            u = readers(v, 1)
+            if u and insts[u[0]].op in ("Relu", "Tanh", "Sigmoid"):
+                return insts[u[0]].op, u
+            if u and insts[u[0]].op == "Gelu":
+                return ("GeluTanh" if insts[u[0]].attrs.get("approximate", "none") in ("tanh", b"tanh") else "Gelu"), u
+            u = readers(v, 2)
+            for s, m in (u, u[::-1]) if u else ():
+                if s != m and insts[s].op == "Sigmoid" and insts[m].op == "Mul" and sorted(insts[m].inputs) == sorted([v, insts[s].outputs[0]]) \
+                        and readers(insts[s].outputs[0], 1):
+                    return "Swish", [s, m]
+            return None, []
+
+        def take_residual(v):
+            u = readers(v, 1)
+            if u and insts[u[0]].op == "Add":
+                other = [t for t in insts[u[0]].inputs if t != v]
+                if len(other) == 1 and other[0] not in consts:
+                    return other[0], u
+            return "", []
+
+        act, residual, first = None, "", False
+        if epilogue:
+            act, u = take_activation(v)
+            if u:
+                chain, v = chain + u, insts[u[-1]].outputs[0]
+            residual, u = take_residual(v)
+            if u:
+                chain, v = chain + u, insts[u[0]].outputs[0]
+                if act is None:
+                    act, u = take_activation(v)
+                    if u:
+                        first, chain, v = True, chain + u, insts[u[-1]].outputs[0]
+        name = i.inputs[1] + "@rows"
+        added[name] = np.ascontiguousarray(w if trans else w.T)
+        dropped.add(i.inputs[1])
+        taken.update(chain)
+        replaced[chain[-1]] = Inst("Linear", [i.inputs[0], name, bias, residual], [v], activation=act, residual_first=first, weights=i.inputs[1], trans=trans,
+                                   bias_dims=np.asarray(consts[bias]).ndim if bias else 0, members=[insts[c] for c in chain])
+    if not replaced:
+        return program
+    new = [replaced.get(k, i) for k, i in enumerate(insts) if k in replaced or k not in taken]
+    used = {v for i in new for v in i.inputs} | set(program.outputs)
+    constants = {k: v for k, v in consts.items() if k not in dropped or k in used}
+    constants.update(added)
+    return Program(_topological(new, set(constants) | set(program.inputs)), constants, program.inputs, program.outputs)
+
+
 # ---- elementwise fusion over a program -----------------------------------------------------------------------------------
 _NP_NAME = {np.dtype(np.float32): "float32", np.dtype(np.float64): "float64", np.dtype(np.float16): "float16", np.dtype(np.int8): "int8",
             np.dtype(np.uint8): "uint8", np.dtype(np.int32): "int32", np.dtype(np.int64): "int64", np.dtype(np.bool_): "bool", np.dtype(np.int16): "int16"}
@@ -378,6 +481,14 @@ def infer_dtypes(program):
             o = ["float32", "uint8"]
         elif inst.op == "Shape":
             o = ["int64"]
+        elif inst.op == "LayerNormalization":
+            o = [first, "float32", "float32"]
+        elif inst.op == "LayerNormalizationGrad":
+            o = [dt.get(inst.inputs[1], "float32")] + [dt.get(inst.inputs[2], "float32")] * 2
+        elif inst.op == "TokenLogProbs":
+            o = ["float32"] * 4 + ["int64"]
+        elif inst.op == "TokenLogProbsGrad":
+            o = [dt.get(inst.inputs[2], "float32")]
         else:
             o = [first] * len(inst.outputs)
         for name, d in zip(inst.outputs, o):
@@ -467,6 +578,11 @@ def program_to_onnx(program, name="graph"):
         elif i.op == "ElementWiseNvrtc":
             for op, ins, outs in i.attrs["members"]:
                 nodes.append(N(op, ins, outs, {}))
+        elif i.op == "Linear":
+            w = np.asarray(consts[i.inputs[1]])
+            consts[i.attrs["weights"]] = w if i.attrs["trans"] else np.ascontiguousarray(w.T)
+            for m in i.attrs["members"]:
+                nodes.append(N(m.op, m.inputs, m.outputs, dict(m.attrs)))
         elif i.op == "QLinearConv" and (i.attrs.get("quantize_input") or i.attrs.get("pool")):
             skip = ("quantize_input", "quantized_name", "pool", "conv_output")
             attrs = {k: v for k, v in i.attrs.items() if k not in skip and v is not None and not (isinstance(v, (list, tuple)) and len(v) == 0)}
@@ -834,6 +950,36 @@ class Executor:
         elif op == "Flatten":
             ax = a.get("axis", 1)
             env[out] = x[0].reshape(int(np.prod(x[0].shape[:ax])), -1)
+        elif op == "Linear":
+            dims = a["bias_dims"]  # a bias [1, O] gives the product of a vector a row
+            xin = x[0].reshape((1,) * (dims - x[0].dim()) + tuple(x[0].shape)) if x[0].dim() < dims else x[0]
+            env[out] = self._linear(xin, x[1], x[2].reshape(-1) if has(2) else None, a["activation"], x[3], a["residual_first"])
+        elif op == "LayerNormalization":
+            if int(a.get("stash_type", 1)) != 1:
+                raise NotImplementedError("LayerNormalization: stash_type must be 1 (statistics in 32 bits)")
+            y = ops.LayerNormalization(x[0], x[1], x[2] if has(2) else None, axis=a.get("axis", -1), epsilon=a.get("epsilon", 1e-5), stats=len(inst.outputs) > 1)
+            for name, v in zip(inst.outputs, y if len(inst.outputs) > 1 else (y,)):
+                env[name] = v
+        elif op == "LayerNormalizationGrad":
+            for name, v in zip(inst.outputs, ops.LayerNormalizationGrad(x[0], x[1], x[2], x[3], x[4], axis=a.get("axis", -1))):
+                env[name] = v
+        elif op == "TokenLogProbs":
+            for name, v in zip(inst.outputs, ops.TokenLogProbs(x[0], x[1], a.get("num_top", 0), a.get("ignore_index"))):
+                env[name] = v
+        elif op == "TokenLogProbsGrad":
+            env[out] = ops.TokenLogProbsGrad(x[0] if has(0) else None, x[1] if has(1) else None, x[2], x[3], x[4], x[5] if has(5) else None, a.get("ignore_index"))
+        elif op == "SoftmaxCrossEntropyLoss":
+            if has(2) or len(inst.outputs) > 1:
+                raise NotImplementedError("SoftmaxCrossEntropyLoss with class weights or its second output")
+            ignore, reduction = a.get("ignore_index"), a.get("reduction", "mean")
+            loss = -ops.TokenLogProbs(x[0].movedim(1, -1), x[1], 0, ignore)[0]
+            if reduction == "sum":
+                loss = loss.sum()
+            elif reduction == "mean":
+                loss = loss.mean() if ignore is None else loss.sum() / (x[1] != ignore).sum()
+            env[out] = loss.to(x[0].dtype)
+        elif op == "Gelu":
+            env[out] = t.nn.functional.gelu(x[0], approximate="tanh" if a.get("approximate", "none") in ("tanh", b"tanh") else "none")
         elif op == "Gemm" and a.get("transB", 0) and not a.get("transA", 0) and a.get("alpha", 1.0) == 1.0 and a.get("beta", 1.0) == 1.0 \
                 and x[0].dtype == t.float32 and x[0].dim() == 2:
             env[out] = ops.Linear(x[0].contiguous(), x[1].contiguous(), x[2] if has(2) else None)  # the classifier of a quantized CNN
@@ -859,6 +1005,27 @@ class Executor:
                 env[out] = y + a.get("beta", 1.0) * x[2] if len(x) > 2 else y
         else:
             raise NotImplementedError("run_onnx: op %s" % op)
+
+    def _linear(self, x, w, b, activation, residual, residual_first):
+        """A Linear instruction.  An Add may broadcast: a residual of another shape (known at run time) is added behind the kernel."""
+        t, ops = self.torch, self.ops
+        if residual is None or (tuple(residual.shape) == tuple(x.shape[:-1]) + (w.shape[0],) and residual.dtype == x.dtype):
+            return ops.Linear(x, w, b, activation=activation, residual=residual, residual_first=residual_first)
+        y = ops.Linear(x, w, b, activation=None if residual_first else activation) + residual
+        if not residual_first or activation is None:
+            return y
+        f = t.nn.functional
+        return {"Relu": t.relu, "Tanh": t.tanh, "Sigmoid": t.sigmoid, "Gelu": f.gelu, "GeluTanh": lambda v: f.gelu(v, approximate="tanh"), "Swish": f.silu}[activation](y)
+
+    def top(self, y, expected=None, k=1):
+        """The k most probable entries along the last dimension of a float output, by TokenLogProbs: their indices and log
+        probabilities [rows][k] and, where the expected values are given, the log probability of each row's largest one."""
+        t = self.torch
+        v = y.shape[-1]
+        tokens = t.zeros(y.shape[:-1], dtype=t.int64, device=y.device) if expected is None else self.stage(np.asarray(expected).argmax(axis=-1).astype(np.int64))
+        lp, _, _, top_lp, top = self.ops.TokenLogProbs(y, tokens, min(k, v))
+        k = min(k, v)
+        return top.reshape(-1, k).tolist(), top_lp.reshape(-1, k).tolist(), None if expected is None else lp.reshape(-1).tolist()
 
     def _stem(self, inst, x, sc, has, strides, pads, group, auto_pad, fq, fpool):
         """The fused forms of a stem convolution (QuantizeLinear in front and / or MaxPool behind); None when the library has no
@@ -946,6 +1113,7 @@ def parse_args(argv):
     ap.add_argument("--host_scalars", action="store_true",
                     help="read dynamic-quantization scales and zero points back to the host per operator, as the reference's VM does; "
                          "default: they stay on the device (same results, no synchronization, the program can be captured in a CUDA graph)")
+    ap.add_argument("--top", type=int, default=0, metavar="K", help="report the K most probable entries of every float output's last dimension (at most 32)")
     ap.add_argument("--no_peephole", action="store_true")
     ap.add_argument("--fuse_operations", action="store_true")
     ap.add_argument("--use_nvrtc", action="store_true")
@@ -968,8 +1136,10 @@ def run_onnx(argv):
     sys.path.insert(0, ROOT)
     import __graft_entry__ as entry
     entry.load_package()
-    from chainer_compiler_b200 import onnx_io
+    from chainer_compiler_b200 import _lib, onnx_io
     args = parse_args(argv)
+    if not 0 <= args.top <= _lib.MAX_TOP:
+        raise SystemExit("run_onnx: --top must be between 0 and %d" % _lib.MAX_TOP)
     if args.backend != "chxvm":
         raise SystemExit("run_onnx: unknown backend %r (this package has the chxvm backend only)" % args.backend)
     target = args.test or args.onnx or args.positional
@@ -980,7 +1150,7 @@ def run_onnx(argv):
     else:
         model, cases = onnx_io.load_model(target), []
     unfused = compile_model(model, quantize=args.quantize, per_channel=not args.disable_per_channel_quantize, fold_bn_first=args.fold_bn_first,
-                            peephole=not args.no_peephole)
+                            peephole=not args.no_peephole, float_linear=not args.float_ops_via_torch)
     # the reference fuses for NVRTC only when both flags are given (compiler/passes.cc: fusion needs a code generator)
     program = fuse_elementwise(unfused) if (args.fuse_operations and args.use_nvrtc) else unfused
     if args.dump_onnx or args.out_onnx:
@@ -1018,6 +1188,17 @@ def run_onnx(argv):
             if it > 0 or args.iterations == 1:  # the first iteration is discarded when there are several (tools/run_onnx.cc:468-469)
                 elapsed.append(time.perf_counter() - t0)
         got = {k: v.detach().cpu().numpy() for k, v in outs}
+        tops = {}
+        if args.top:
+            want_of = dict(expected)
+            for name, v in outs:
+                if v.dim() >= 1 and v.numel() and v.dtype in (torch.float32, torch.float16):
+                    w = want_of.get(name)
+                    idx, lps, exp = tops[name] = ex.top(v, w if w is not None and w.shape == tuple(v.shape) else None, args.top)
+                    if not args.quiet:
+                        for r in range(len(idx)):
+                            print("case %d output %s row %d: %s%s" % (ci, name, r, ", ".join("%d (%.4f)" % p for p in zip(idx[r], lps[r])),
+                                                                      "" if exp is None else "; expected: %.4f" % exp[r]))
         if args.dump_outputs_dir:
             os.makedirs(args.dump_outputs_dir, exist_ok=True)
             for pc, inst in enumerate(program.insts):
@@ -1040,6 +1221,8 @@ def run_onnx(argv):
             if not ok:
                 failures += 1
             report.append({"case": ci, "output": name, "ok": bool(ok)})
+            if name in tops:
+                report[-1]["top"] = dict(zip(("indices", "logprobs", "expected"), tops[name]))
         if args.verbose and not args.quiet:
             print("case %d: %s" % (ci, {k: v.shape for k, v in got.items()}))
     if tracer is not None:
