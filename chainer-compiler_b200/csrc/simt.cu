@@ -7,6 +7,7 @@
 #include "common.h"
 #include "epilogue.cuh"
 #include "kernels.h"
+#include "linear_chain.cuh"
 #include "pdl.cuh"
 
 namespace chxq {
@@ -890,13 +891,37 @@ extern "C" int chxq_global_avgpool_dq_nhwc(const uint8_t* x, int32_t N, int32_t 
     return CHXQ_OK;
 }
 
+// Products for which the pipelined tiles are too small.  The kernels by what an SM has to do, in thousandths of a microsecond per 2048 k and output: 12 in
+// 128 x 128 blocks and 13.5 in 128 x 64, 17 where there is one block per SM, and 19.5 in the 32 x 64 blocks of linear_f32_regs_kernel, which there are
+// more of.  One B200, in us as 32 x 64, 128 x 64 and 128 x 128: [2048, 2048] x [2048, 2048]^T 532, 447, 401; [349, 4686] x [3125, 4686]^T 396, 318, 627;
+// [1024, 1000] x [1000, 1000]^T 76, 73, 115; [512, 19] x [1500, 19]^T 5.6, 6.9, 11.0; [30, 333] x [10000, 333]^T 19.9, 45, 42.
+static void launch_linear_large(const float* x, const float* w, const float* b, int N, int K, int O, float* y, bool rows16, cudaStream_t s) {
+    auto blocks = [&](int bm, int bn) { return (int64_t)((N + bm - 1) / bm) * ((O + bn - 1) / bn); };
+    auto cost = [&](int bm, int bn, double one, double more) { return (blocks(bm, bn) + 147) / 148 * bm * bn * (blocks(bm, bn) > 148 ? more : one); };
+    const double small = cost(32, 64, 19.5, 19.5), wide = cost(128, 64, 17, 13.5), large = cost(128, 128, 17, 12);
+    if (small <= wide && small <= large) {
+        linear_f32_regs_kernel<<<dim3((O + 63) / 64, (N + 31) / 32), kLinThreads, 0, s>>>(x, w, b, N, K, O, y);
+    } else if (wide <= large) {
+        auto* kernel = rows16 ? linear_chain_kernel<8, 4, 4> : linear_chain_kernel<8, 4, 1>;
+        kernel<<<dim3((O + 63) / 64, (N + 127) / 128), 256, 0, s>>>(x, w, b, N, K, O, y);
+    } else {
+        auto* kernel = rows16 ? linear_chain_kernel<8, 8, 4> : linear_chain_kernel<8, 8, 1>;
+        kernel<<<dim3((O + 127) / 128, (N + 127) / 128), 256, 0, s>>>(x, w, b, N, K, O, y);
+    }
+}
+
 extern "C" int chxq_linear_f32(const float* x, const float* w, const float* b, int32_t N, int32_t K, int32_t O, float* y, void* stream) {
     CHXQ_CHECK_ARG(x && w && y && N > 0 && K > 0 && O > 0, "Linear: bad arguments");
+    constexpr int kMostRows = 65535 * 32;  // of one launch
+    for (; N > kMostRows; N -= kMostRows, x += (int64_t)kMostRows * K, y += (int64_t)kMostRows * O) {
+        const int rc = chxq_linear_f32(x, w, b, kMostRows, K, O, y, stream);
+        if (rc != CHXQ_OK) return rc;
+    }
     // The largest register tile that still puts a block on every second SM (4 x 4: 2048 outputs per block), and for few outputs the
     // single-output tile, whose chains are the shortest, as long as no SM has more than two blocks of it at a time.  Lines from 1338 shapes on
     // one B200, in us: K = 2048, O = 1000: 192 rows 49.5 as 4 x 4 and 51.7 as 2 x 2, 128 rows 49.4 and 41.2; [16, 512] x [1000, 512]^T 6.4 as 1 x 1
-    // and 8.9 as 2 x 2, [40, 512] 14.6 and 8.9, [24, 66] x [1000, 66]^T 5.6 and 5.3 (K <= 64 is over before slices of 128 pay).  The kernel with
-    // registers takes what the pipelined tiles do not win: more than two 4 x 4 blocks per SM, K < 400 there, rows that are no whole 16-byte
+    // and 8.9 as 2 x 2, [40, 512] 14.6 and 8.9, [24, 66] x [1000, 66]^T 5.6 and 5.3 (K <= 64 is over before slices of 128 pay).  The kernels with
+    // registers take what the pipelined tiles do not win: more than two 4 x 4 blocks per SM, K < 400 there, rows that are no whole 16-byte
     // pieces, and from 80,000 outputs on K <= 32 ([40, 32] x [4000, 32]^T 5.2 against 6.4).
     const int64_t outputs = (int64_t)N * O;
     const bool rows16 = K % 4 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15u) == 0;
@@ -909,7 +934,7 @@ extern "C" int chxq_linear_f32(const float* x, const float* w, const float* b, i
     else if (two_per_sm(64, 32) && rows16 && K >= 400)
         CHXQ_CUDA((launch_linear<LinTile<4, 4, 8, 64, 4, 2>>(x, w, b, N, K, O, y, s)));
     else
-        linear_f32_regs_kernel<<<dim3((O + 63) / 64, (N + 31) / 32), kLinThreads, 0, s>>>(x, w, b, N, K, O, y);
+        launch_linear_large(x, w, b, N, K, O, y, rows16, s);
     CHXQ_LAUNCH_CHECK();
     return CHXQ_OK;
 }

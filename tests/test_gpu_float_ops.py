@@ -92,6 +92,26 @@ def test_linear_few_rows_of_fp32(ops, dev, m, k, o, pitch):
     _check_linear(ops, dev, m, k, o, torch.float32, "Tanh", "first" if m % 2 else "last", pitch=pitch)
 
 
+@pytest.mark.parametrize("m,k,o", [(2048, 64, 2000), (1900, 17, 2100), (349, 500, 3125), (1024, 33, 1000), (300, 40, 5000), (65, 300, 20000), (2200000, 3, 2)])
+def test_linear_fp32_without_an_epilogue_is_one_chain(ops, dev, m, k, o):
+    """y = b + a chain of fused multiply-adds in ascending k, in large products as in small ones: sampled outputs, bit for bit."""
+    g = torch.Generator(device=dev).manual_seed(m + k + o)
+    x, w, b = torch.randn((m, k), device=dev, generator=g), torch.randn((o, k), device=dev, generator=g), torch.randn(o, device=dev, generator=g)
+    y = ops.Linear(x, w, b)
+    rows = torch.cat([torch.tensor([0, m - 1, m // 2], device=dev), torch.randint(0, m, (29,), device=dev, generator=g)])
+    cols = torch.cat([torch.tensor([0, o - 1], device=dev), torch.randint(0, o, (30,), device=dev, generator=g)])
+    got = y[rows][:, cols].cpu()
+    xs, ws = x[rows].cpu(), w[cols].cpu()
+    acc = torch.zeros((32, 32))
+    for i in range(k):  # (a product of two fp32 values is exact in 64 bits; its sum rounds to 64 and then to 32, which is one rounding but next to a tie)
+        acc = (xs[:, i:i + 1].double() * ws[:, i].double() + acc.double()).float()
+    want = acc + b[cols].cpu()
+    assert torch.equal(got, ops.Linear(x[rows], w[cols], b[cols]).cpu())  # another kernel
+    # a tie decided the other way moves a chain by a unit in the last place of its value then
+    mag = xs.double().abs() @ ws.double().abs().t() + b[cols].cpu().double().abs()
+    assert (got == want).float().mean() > 0.99 and ((got.double() - want.double()).abs() <= k * E32 * mag).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_offset_addresses_and_other_strides(ops, dev, dtype):
     """Operands that start off a 16-byte boundary, a transposed weight, rows that overlap (an expanded one), a batch of leading dimensions."""
