@@ -732,7 +732,8 @@ bool same_places(uintptr_t bits, int64_t rows, int64_t ld, int64_t other, int ve
 
 template <typename F, typename... Args>
 int launch_rows(F* kernel, const Plan& p, size_t smem, cudaStream_t s, Args... args) {
-    if (smem > 40 * 1024) CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (always the same limit, that of the longest rows: another thread may be between this and its launch)
+    if (smem > 48 * 1024) CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
     CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)p.blocks), p.G * p.groups, smem, s, args...));
     count_launch(1);
     return CHXQ_OK;
@@ -794,9 +795,14 @@ extern "C" int chxq_layernorm(const void* x, int64_t ldx, int32_t dtype, const v
     });
 }
 
+// Shares of the parameters' sums: one per block, and fewer of rows that are longer than blocks take, 39 MB in all.
+static int grad_shares(int64_t D) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(kMaxBlocks, (int64_t)kMaxBlocks * 32768 / D));
+}
+
 extern "C" size_t chxq_layernorm_grad_workspace(int64_t rows, int64_t D) {
     if (rows < 0 || D < 1) return 0;
-    return (size_t)kMaxBlocks * 2 * (size_t)D * sizeof(float);
+    return (size_t)grad_shares(D) * 2 * (size_t)D * sizeof(float);
 }
 
 extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype, const void* scale, int32_t affine_dtype,
@@ -833,13 +839,14 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
                 shares = p.blocks;
                 if (p.G > 32) {
                     const int row_bytes = (int)share * 16;
-                    const int room = 220 * 1024, stages = std::min(kMaxStages, room / (p.groups * 2 * row_bytes));
+                    constexpr int room = 220 * 1024;  // (the limit is set to it, whatever a call needs: another thread may be between that and its launch)
+                    const int stages = std::min(kMaxStages, room / (p.groups * 2 * row_bytes));
                     // the groups' sums are not laid out by row but by piece: also those of pieces that hold no column
                     const size_t smem = std::max((size_t)stages * p.groups * 2 * row_bytes, (size_t)2 * share * VEC * sizeof(float));
                     int* status = device_status_ptr();
                     if (!status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
                     auto go = [&](auto* kernel) {
-                        CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                        CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room));
                         CHXQ_CUDA(launch_pdl_cluster(cl, kernel, dim3((unsigned)(p.blocks * cl)), p.G * p.groups, smem, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D,
                                                      p.G, stages, row_bytes, static_cast<T*>(dx), part, status, (uint64_t)tc::wait_limit_ns_value()));
                         count_launch(1);
@@ -866,7 +873,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
             }
             layernorm_dx_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kThreads, 0, s>>>(g, lddy, v, ldx, sc, mean, inv_std_dev, rows, D, static_cast<T*>(dx));
             CHXQ_LAUNCH_CHECK();
-            shares = (int)std::min<int64_t>(rows, 148);
+            shares = (int)std::min<int64_t>(rows, grad_shares(D));
             layernorm_dparam_long_kernel<T><<<dim3((unsigned)((D + kThreads - 1) / kThreads), shares), kThreads, 0, s>>>(g, lddy, v, ldx, mean, inv_std_dev, rows, D, part);
             CHXQ_LAUNCH_CHECK();
             return CHXQ_OK;

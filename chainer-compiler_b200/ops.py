@@ -294,7 +294,8 @@ def LayerNormalization(x, scale, bias=None, axis=-1, epsilon=1e-5, stats=False):
 
 def LayerNormalizationGrad(dy, x, scale, mean, inv_std_dev, axis=-1):
     """Gradient of LayerNormalization: (dx, dscale, dbias) from the gradient dy of y and the statistics that the forward call returned.
-    dscale and dbias have scale's type; they are sums over all rows, taken in 32 bits in an order that depends on the sizes alone."""
+    dscale and dbias have scale's type; they are sums over all rows, taken in 32 bits in an order that depends on sizes, strides and
+    alignment alone."""
     return _native.layernorm_grad(dy, x, scale, mean, inv_std_dev, axis)
 
 

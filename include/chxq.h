@@ -417,8 +417,8 @@ int chxq_layernorm(const void* x, int64_t ldx, int32_t dtype, const void* scale,
                    float epsilon, void* y, float* mean, float* inv_std_dev, void* stream);
 /* Its gradient.  With xh = (x - mean) inv_std_dev and g = dy scale:
  *   dx = inv_std_dev (g - mean(g) - xh mean(g xh)),  dscale = sum over the rows of dy xh,  dbias = sum over the rows of dy.
- * dx [rows, D] of x's type, dscale and dbias [D] of scale's type; dbias may be NULL.  The order of the sums depends on the extents alone:
- * the same call gives the same bits. */
+ * dx [rows, D] of x's type, dscale and dbias [D] of scale's type; dbias may be NULL.  The order of the sums depends on extents, pitches and
+ * alignment alone: the same call gives the same bits. */
 size_t chxq_layernorm_grad_workspace(int64_t rows, int64_t D);
 int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype, const void* scale, int32_t affine_dtype,
                         const float* mean, const float* inv_std_dev, int64_t rows, int64_t D, void* dx, void* dscale, void* dbias, void* workspace,

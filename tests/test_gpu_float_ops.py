@@ -271,11 +271,46 @@ def test_layernorm_grad_extents(ops, dev, dtype, rows, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,d", [(20001, 520), (6001, 1030), (3001, 4999), (2405, 8192), (1501, 12001), (1203, 16384), (803, 28000)])
+@pytest.mark.parametrize("rows,d", [(20001, 520), (6001, 1030), (3001, 4999), (2405, 8192), (1501, 12001), (1203, 16384), (803, 28000), (171, 70001)])
 def test_layernorm_grad_of_many_rows(ops, dev, dtype, rows, d):
     """More rows than a block holds at once, several times over: what holds the rows is filled again and again, and no wait runs out."""
     _check_grad(ops, dev, rows, d, dtype, dtype)
     ops.device_status()
+
+
+def test_calls_from_two_threads(ops, dev):
+    """Threads with a stream each call the same operators with other sizes, which need other amounts of shared memory, at the same time."""
+    import threading
+
+    g = torch.Generator(device=dev).manual_seed(9)
+    cases = []
+    for rows, d in ((300, 520), (200, 8192), (150, 4999), (90, 64)):
+        x, dy = (torch.randn((rows, d), device=dev, generator=g) for _ in range(2))
+        s = torch.randn(d, device=dev, generator=g)
+        w = torch.randn((256, d), device=dev, generator=g)
+        y, mean, inv = ops.LayerNormalization(x, s, stats=True)
+        cases.append((x, dy, s, w, mean, inv, ops.LayerNormalizationGrad(dy, x, s, mean, inv), ops.Linear(y, w, activation="Tanh")))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in order * 25:
+                    x, dy, s, w, mean, inv, want, z = cases[k]
+                    got = ops.LayerNormalizationGrad(dy, x, s, mean, inv)
+                    y = ops.LayerNormalization(x, s)
+                    if not (all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(ops.Linear(y, w, activation="Tanh"), z)):
+                        bad.append(k)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in ([0, 1, 2, 3], [3, 2, 1, 0], [1, 0, 3, 2])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_layernorm_grad_against_differences(ops, dev):
