@@ -213,10 +213,10 @@ int launch_tc(const chxq_linear_params& q, const Operands& op, const lin::TcArgs
 
 template <>
 int launch_tc<float>(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
-    if (q.M <= 16) return launch_tile_32<16, 4>(q, op, args, s);
-    if (q.M <= 32) return launch_tile_32<32, 4>(q, op, args, s);
-    if (q.M <= 64) return launch_tile_32<64, 4>(q, op, args, s);
-    return launch_tile_32<128, 3>(q, op, args, s);
+    if (q.M <= 16) return launch_tile_32<16, 6>(q, op, args, s);
+    if (q.M <= 32) return launch_tile_32<32, 6>(q, op, args, s);
+    if (q.M <= 64) return launch_tile_32<64, 6>(q, op, args, s);
+    return launch_tile_32<128, 4>(q, op, args, s);
 }
 
 // A few rows of fp32.  No alignment is asked for: rows off 16-byte boundaries are read value by value ([1, 2147] x [2999, 2147]^T: 8 us, and 27 with copies in

@@ -34,18 +34,29 @@ __host__ __device__ constexpr uint32_t idesc_extents(int m, int n) {
 __host__ __device__ constexpr uint32_t idesc_tf32() {
     return (1u << 4) | (2u << 7) | (2u << 10);
 }
-__device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A B^T over eight values of K, A in tensor memory: a row a lane, a value a column.
+__device__ __forceinline__ void umma_tf32(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
             "{\n\t"
             ".reg .pred p;\n\t"
-            ".reg .b64 da, db;\n\t"
-            "mov.b64 da, {%1, %3};\n\t"
+            ".reg .b64 db;\n\t"
             "mov.b64 db, {%2, %3};\n\t"
             "setp.ne.b32 p, %5, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::tf32 [%0], da, db, %4, p;\n\t"
+            "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], db, %4, p;\n\t"
             "}\n" ::"r"(tmem_d),
-            "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+            "r"(tmem_a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
             : "memory");
+}
+
+// Sixteen columns of the warp's 32 lanes of tensor memory.
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // D[tmem] (+)= A B^T over 32 bytes of K of each operand, kind::f16, issued by one thread; PAIR: over a CTA pair (M = 256).

@@ -228,37 +228,56 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant_
 // The tensor cores multiply tf32, eleven significant bits.  A value is split as a = h + l with h = tf32(a) and l = tf32(a - h), rounded to nearest, and the
 // product taken as h h' + h l' + l h': what is left out is below 2^-21 |a a'|, the rounding of an fp32 product in a sum of a few.
 // The sums: h h' goes through TMEM in chains of kChain K blocks (at most 16 instructions, whose additions the tensor core may truncate), each then
-// added in registers; the two small products have an accumulator of their own, 2^-11 in size, for the whole of K.  [2048, 2048] x [2048, 2048]^T: 140
-// us, 3.5e-7 off the sums in 64 bits (root mean square, relative); chains of eight 138 us and 6.4e-7, of two 147 us and 2.2e-7; an fp32 product 8.1e-7.
-// Roles as above, with 640 threads: warps 0 and 2 load, warp 1 issues, warps 4-19 split each stage as it arrives (h in place, l beside it; the swizzle does
-// not matter to an elementwise pass), drain the chains and run the epilogue.
-// Bound: the instructions of the splitting (twenty-six per sixteen bytes; with eight warps their latency: 163 us for 2048^3) and shared memory.
+// added in registers; the two small products have an accumulator of their own, 2^-11 in size, for the whole of K.  [2048, 2048] x [2048, 2048]^T:
+// 3.5e-7 off the sums in 64 bits (root mean square, relative); chains of eight 6.4e-7 for 2% less time, of two 2.2e-7 for 5% more; an fp32
+// product 8.1e-7.
+// The operands: w is split into tensor memory, two stages of h and l, x in place in shared memory with l beside it.  (Both in shared memory: 192 KB of
+// traffic a K block instead of 112, 140 us for 2048^3 where this takes 109.)  h and l of x are neighbours, so that one instruction of 2 BN columns
+// takes h of w times both: h h' into the chain's accumulator and h l' into the small products'.  Those lie between the accumulators of even and of odd
+// chains, and x's halves change places with the chain.  Since the instruction adds to both or to none, a chain starts from zeros that are written.
+// Roles as above, with 640 threads: warps 0 and 2 load, warp 1 issues, warps 4-19 split, in two groups that take the K blocks by turns, drain the chains and
+// run the epilogue.
+// Bound: a K block of 128 x 128 takes 0.8 us where the tensor pipe needs 0.41: the splitting (some twenty-three instructions per sixteen bytes) and the
+// issuing thread (eight products and a commit of 75 to 90 cycles each beside busy warps).
 template <int BN, int STAGES>
 struct TileF32Config {
-    static constexpr int kTileW = 128 * 128, kTileX = BN * 128, kRaw = kTileW + kTileX, kStage = 2 * kRaw;
+    static constexpr int kTileW = 128 * 128, kTileX = BN * 128, kStage = kTileW + 2 * kTileX;
     static constexpr int kSums = BN * 128 * 4;
     static constexpr int kData = STAGES * kStage > kSums ? STAGES * kStage : kSums;
     static constexpr int kNumBars = 3 * STAGES + 5;
     static constexpr int kSmem = 1024 + kData + kNumBars * 8 + 16;
     static constexpr int kChain = 4;  // K blocks of 32 values
-    static constexpr int kTmemCols = 3 * BN <= 64 ? 64 : (3 * BN <= 128 ? 128 : (3 * BN <= 256 ? 256 : 512));
+    static constexpr int kTmemW = 3 * BN;  // first column of two stages of w, 32 columns of h and 32 of l each
+    static constexpr int kTmemCols = kTmemW + 128 <= 256 ? 256 : 512;
     static_assert(kSmem <= 227 * 1024, "shared memory over the per-CTA limit");
 };
 
-// v = h + l + a rest below 2^-22 |v|, by integer rounding (the conversion instruction runs at a sixteenth of the rate: 279 us where this takes 140 for
-// 2048^3).  Not for what rounds to infinity, infinities and NaN.
-__device__ __forceinline__ void split_tf32(uint32_t v, uint32_t& h, uint32_t& l) {
-    h = (v + 0x1000u) & 0xffffe000u;
-    l = (__float_as_uint(__uint_as_float(v) - __uint_as_float(h)) + 0x1000u) & 0xffffe000u;
-}
-__device__ __forceinline__ bool rounds_away(uint32_t v) {  // to infinity, or it is one or NaN
-    return !(fabsf(__uint_as_float(v)) < __uint_as_float(0x7f7ff000u));
-}
+// v = h + l + a rest below 2^-22 |v|, by integer rounding (the conversion instruction runs at a sixteenth of the rate: 279 us where this took 140 for 2048^3).
+// What rounds to infinity, infinities and NaN: the difference times zero is NaN there, and those four values are done again.
 __device__ __forceinline__ void split_tf32_special(uint32_t v, uint32_t& h, uint32_t& l) {
     const uint32_t a = v & 0x7fffffffu;
     if (a < 0x7f7ff000u) return;
     h = a > 0x7f800000u ? 0x7fffffffu : v & 0xffffe000u;  // NaN; infinity, or cut off instead of rounded
     l = a >= 0x7f800000u ? 0u : __float_as_uint(__uint_as_float(v) - __uint_as_float(h)) & 0xffffe000u;
+}
+__device__ __forceinline__ void split_tf32(const uint4& v, uint32_t* h, uint32_t* l) {
+    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+    f32x2 z = 0ull;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        h[j] = (in[j] + 0x1000u) & 0xffffe000u;
+        h[j + 1] = (in[j + 1] + 0x1000u) & 0xffffe000u;
+        const f32x2 d = add2(make_x2(__uint_as_float(in[j]), __uint_as_float(in[j + 1])), make_x2(-__uint_as_float(h[j]), -__uint_as_float(h[j + 1])));
+        z = fma2(d, 0ull, z);
+        const float2 f = split_x2(d);
+        l[j] = (__float_as_uint(f.x) + 0x1000u) & 0xffffe000u;
+        l[j + 1] = (__float_as_uint(f.y) + 0x1000u) & 0xffffe000u;
+    }
+    const float2 zf = split_x2(z);
+    if (!(zf.x + zf.y == 0.f)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_tf32_special(in[j], h[j], l[j]);
+    }
 }
 
 template <int BN, int STAGES>
@@ -272,17 +291,17 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };
-    auto ready = [&](int s) { return bar0 + 8u * (STAGES + s); };  // split into h and l
+    auto ready = [&](int s) { return bar0 + 8u * (STAGES + s); };  // split into h and l, w in tensor memory
     auto empty = [&](int s) { return bar0 + 8u * (2 * STAGES + s); };
     auto cfull = [&](int b) { return bar0 + 8u * (3 * STAGES + b); };       // a chain is complete in its accumulator
-    auto cempty = [&](int b) { return bar0 + 8u * (3 * STAGES + 2 + b); };  // ... and has been drained
+    auto cempty = [&](int b) { return bar0 + 8u * (3 * STAGES + 2 + b); };  // ... and has been drained and cleared
     const uint32_t done = bar0 + 8u * (3 * STAGES + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full(s), 2);
-            mbar_init(ready(s), 16);  // one arrival per splitting warp
+            mbar_init(ready(s), 8);  // one arrival per splitting warp
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -301,7 +320,7 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_ptr;  // accumulators: two chains by turns, then the small products
+    const uint32_t tmem = *tmem_ptr;  // accumulators: even chains, the small products, odd chains; then w
     pdl_launch_dependents();
     pdl_dependency_wait();
 
@@ -312,6 +331,9 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
     const int chains = (blocks + Cfg::kChain - 1) / Cfg::kChain;
     float* sums = reinterpret_cast<float*>(smem);
     bool got = false;
+    // Where x goes in its stage, h in place and l beside it: h first in even chains, last in odd ones.
+    auto x_high = [](int kb) { return Cfg::kTileW + (kb / Cfg::kChain & 1) * Cfg::kTileX; };
+    auto x_low = [](int kb) { return Cfg::kTileW + (~(kb / Cfg::kChain) & 1) * Cfg::kTileX; };
 
     if (warp < 4) {
         if (lane == 0 && (warp == 0 || warp == 2)) {
@@ -322,14 +344,14 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
                 uint8_t* st = smem + s * Cfg::kStage;
                 mbar_expect_tx(full(s), is_w ? Cfg::kTileW : Cfg::kTileX);
                 if (is_w) tma_load_2d(smem_u32(st), &tmW, full(s), (kb0 + kb) * 128, w0);
-                else tma_load_2d(smem_u32(st + Cfg::kTileW), &tmX, full(s), (kb0 + kb) * 128, x0);
+                else tma_load_2d(smem_u32(st + x_high(kb)), &tmX, full(s), (kb0 + kb) * 128, x0);
             }
         } else if (lane == 0 && warp == 1) {
             bool ok = true;
-            const uint32_t hi = kmajor_desc_hi<128>(), idesc = idesc_tf32() | idesc_extents(128, BN);
+            const uint32_t hi = kmajor_desc_hi<128>(), wide = idesc_tf32() | idesc_extents(128, 2 * BN), narrow = idesc_tf32() | idesc_extents(128, BN);
             for (int kb = 0; kb < blocks; ++kb) {
                 const int s = kb % STAGES, c = kb / Cfg::kChain, in = kb % Cfg::kChain;
-                if (in == 0 && !mbar_wait(cempty(c & 1), ((uint32_t)(c >> 1) & 1u) ^ 1u, abort_flag, p.status, 62, 0, p.wait_limit_ns)) {
+                if (in == 0 && !mbar_wait(cempty(c & 1), (uint32_t)(c >> 1) & 1u, abort_flag, p.status, 62, 0, p.wait_limit_ns)) {
                     ok = false;
                     break;
                 }
@@ -338,13 +360,12 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
                     break;
                 }
                 tc_fence_after();
-                const uint32_t st = smem_u32(smem + s * Cfg::kStage);
-                const uint32_t ah = kmajor_desc_lo(st), bh = kmajor_desc_lo(st + Cfg::kTileW), al = kmajor_desc_lo(st + Cfg::kRaw), bl = kmajor_desc_lo(st + Cfg::kRaw + Cfg::kTileW);
+                const uint32_t both = kmajor_desc_lo(smem_u32(smem + s * Cfg::kStage + Cfg::kTileW)), xh = kmajor_desc_lo(smem_u32(smem + s * Cfg::kStage + x_high(kb)));
+                const uint32_t wh = tmem + (uint32_t)(Cfg::kTmemW + (kb & 1) * 64), wl = wh + 32u;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    umma_tf32(tmem + (uint32_t)((c & 1) * BN), ah + 2u * k, bh + 2u * k, hi, idesc, in > 0 || k > 0 ? 1u : 0u);
-                    umma_tf32(tmem + 2u * BN, ah + 2u * k, bl + 2u * k, hi, idesc, kb > 0 || k > 0 ? 1u : 0u);
-                    umma_tf32(tmem + 2u * BN, al + 2u * k, bh + 2u * k, hi, idesc, 1u);
+                    umma_tf32(tmem + (uint32_t)((c & 1) * BN), wh + 8u * k, both + 2u * k, hi, wide, 1u);
+                    umma_tf32(tmem + (uint32_t)BN, wl + 8u * k, xh + 2u * k, hi, narrow, 1u);
                 }
                 umma_commit(empty(s));
                 if (in == Cfg::kChain - 1 || kb == blocks - 1) umma_commit(cfull(c & 1));
@@ -354,10 +375,10 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
         __syncwarp();
     } else {
         // Warps 4-19: one of four per 32 TMEM lanes (rows of w), and up to four for the columns (rows of x), at least sixteen columns each.
-        const int e = warp - 4, f = (warp & 3) * 32 + lane, part = e >> 2, tid = (int)threadIdx.x - 128;
+        const int e = warp - 4, quarter = (warp & 3) * 32, f = quarter + lane, part = e >> 2;
         constexpr int kParts = BN >= 64 ? 4 : BN / 16, kCols = BN / kParts;
         const bool mine = part < kParts;
-        const uint32_t column0 = (uint32_t)(part * kCols), lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + column0;
+        const uint32_t column0 = (uint32_t)(part * kCols), lanes = tmem + ((uint32_t)quarter << 16) + column0;
         float acc[kCols] = {};
         got = true;
         // Adds columns of TMEM; `finite`: only to sums that are -- next to an infinity the small products are NaN (infinity times l = 0).
@@ -372,53 +393,84 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
                     if (!finite || fabsf(acc[c * 16 + j]) < INFINITY) acc[c * 16 + j] += __uint_as_float(r[j]);
             }
         };
+        // The accumulators start from zeros that are written: an instruction adds to those of a chain and of the small products together.
+        auto clear = [&](uint32_t at) {
+            const uint32_t z[16] = {};
+#pragma unroll
+            for (int c = 0; c < kCols / 16; ++c) tmem_st_32x32b_x16(at + (uint32_t)(c * 16), z);
+        };
+        if (mine) {
+            clear(lanes);
+            clear(lanes + (uint32_t)BN);
+            clear(lanes + 2u * BN);
+            tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(cempty(0));
+            mbar_arrive(cempty(1));
+        }
         auto drain = [&](int c) {  // chain c into the registers; false: gave up
             if (!__all_sync(0xffffffffu, mbar_wait(cfull(c & 1), (uint32_t)(c >> 1) & 1u, abort_flag, p.status, 64, 32, p.wait_limit_ns))) return false;
             tc_fence_after();
-            if (mine) add(lanes + (uint32_t)((c & 1) * BN), false);
+            if (mine) {
+                add(lanes + (uint32_t)((c & 1) * 2 * BN), false);
+                clear(lanes + (uint32_t)((c & 1) * 2 * BN));
+                tmem_st_wait();
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(cempty(c & 1));
             return true;
         };
-        for (int kb = 0; kb < blocks && got; ++kb) {
+        // The warps split in two groups, which take the K blocks by turns: eight warps a block, each 32 rows of w by half of their columns.
+        const int group = part & 1, half = part >> 1, tid = half * 128 + f;
+        int drained = 0;
+        for (int kb = group; kb < blocks && got; kb += 2) {
             const int s = kb % STAGES;
+            // Half a chain on, the one before has been multiplied.
+            if (kb % Cfg::kChain >= Cfg::kChain / 2 && kb % Cfg::kChain < Cfg::kChain / 2 + 2 && kb >= Cfg::kChain && !(got = drain(drained++))) break;
             got = __all_sync(0xffffffffu, mbar_wait(full(s), (uint32_t)(kb / STAGES) & 1u, abort_flag, p.status, 65, 0, p.wait_limit_ns));
             if (!got) break;
-            uint4* raw = reinterpret_cast<uint4*>(smem + s * Cfg::kStage);
-            uint4* low = reinterpret_cast<uint4*>(smem + s * Cfg::kStage + Cfg::kRaw);
-#pragma unroll 4
-            for (int i = tid; i < Cfg::kRaw / 16; i += 512) {
-                const uint4 v = raw[i];
-                uint4 h, l;
-                split_tf32(v.x, h.x, l.x);
-                split_tf32(v.y, h.y, l.y);
-                split_tf32(v.z, h.z, l.z);
-                split_tf32(v.w, h.w, l.w);
-                if (rounds_away(v.x) || rounds_away(v.y) || rounds_away(v.z) || rounds_away(v.w)) {
-                    split_tf32_special(v.x, h.x, l.x);
-                    split_tf32_special(v.y, h.y, l.y);
-                    split_tf32_special(v.z, h.z, l.z);
-                    split_tf32_special(v.w, h.w, l.w);
+            // w: row f, sixteen of the block's 32 columns, into tensor memory; TMA has swizzled the row's pieces
+            const uint4* raw_w = reinterpret_cast<const uint4*>(smem + s * Cfg::kStage) + f * 8;
+            uint32_t wh[16], wl[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split_tf32(raw_w[(4 * half + j) ^ (f & 7)], wh + 4 * j, wl + 4 * j);
+            uint4* raw = reinterpret_cast<uint4*>(smem + s * Cfg::kStage + x_high(kb));
+            uint4* low = reinterpret_cast<uint4*>(smem + s * Cfg::kStage + x_low(kb));
+#pragma unroll
+            for (int j = 0; j < (BN * 8 + 255) / 256; ++j) {
+                const int i = tid + j * 256;
+                if (BN * 8 % 256 == 0 || i < BN * 8) {
+                    uint32_t h[4], l[4];
+                    split_tf32(raw[i], h, l);
+                    raw[i] = make_uint4(h[0], h[1], h[2], h[3]);
+                    low[i] = make_uint4(l[0], l[1], l[2], l[3]);
                 }
-                raw[i] = h;
-                low[i] = l;
             }
+            if (kb >= 2) {  // the block before the last in its place has been multiplied
+                got = __all_sync(0xffffffffu, mbar_wait(empty((kb - 2) % STAGES), (uint32_t)((kb - 2) / STAGES) & 1u, abort_flag, p.status, 67, 0, p.wait_limit_ns));
+                if (!got) break;
+            }
+            tc_fence_after();
+            const uint32_t to = tmem + ((uint32_t)quarter << 16) + (uint32_t)(Cfg::kTmemW + (kb & 1) * 64 + half * 16);
+            tmem_st_32x32b_x16(to, wh);
+            tmem_st_32x32b_x16(to + 32u, wl);
+            tmem_st_wait();
+            tc_fence_before();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(ready(s));
-            // the chain before the one that ends here has long been multiplied
-            if (kb % Cfg::kChain == Cfg::kChain - 1 && kb / Cfg::kChain > 0) got = drain(kb / Cfg::kChain - 1);
         }
-        // what is left: the chain before the last, if its last block did not end a chain, and the last
-        if (got && chains > 1 && blocks % Cfg::kChain != 0) got = drain(chains - 2);
-        if (got) got = drain(chains - 1);
+        while (got && drained < chains) got = drain(drained++);
         if (got) got = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, p.status, 66, 32, p.wait_limit_ns));
         tc_fence_after();
         // Every stage has been read; the warps write the sums together or not at all.
         got = bar_all(1, 512, got);
         if (got && mine) {
-            add(lanes + 2u * BN, true);
+            add(lanes + (uint32_t)BN, true);
 #pragma unroll
             for (int c = 0; c < kCols; ++c) sums[((int)column0 + c) * 128 + f] = acc[c];
         }
