@@ -114,37 +114,16 @@ struct Operands {  // as TMA reads them
     int64_t ldw;
 };
 
-// kernel: one of linear_tile.cuh's, for bn rows of x.
+// kernel: one of linear_tile.cuh's, for bn rows of x, with `split` CTAs for a tile.
 template <typename F>
-int launch_tile(F* kernel, int bn, int threads, int smem, KernelState& st, const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, int size,
-                cudaStream_t s) {
-    int dev = 0, rc = current_device(&dev);
-    if (rc != CHXQ_OK || (rc = set_smem(kernel, smem, st, dev)) != CHXQ_OK) return rc;
+int launch_tile(F* kernel, int bn, int split, int threads, int smem, KernelState& st, int dev, const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args,
+                int size, cudaStream_t s) {
+    int rc = set_smem(kernel, smem, st, dev);
+    if (rc != CHXQ_OK) return rc;
     alignas(64) CUtensorMap tmW, tmX;
     if ((rc = tc::encode_rows_map(&tmW, op.w, q.K * size, q.O, op.ldw * size, 128)) != CHXQ_OK) return rc;
     if ((rc = tc::encode_rows_map(&tmX, op.x, q.K * size, q.M, op.ldx * size, bn)) != CHXQ_OK) return rc;
     const int64_t x_tiles = (q.M + bn - 1) / bn, tiles = x_tiles * ((q.O + 127) / 128);
-    // How many CTAs share a tile.  16-bit kernels, of which an SM holds two: doubled as long as there are no more CTAs than that and each has a K block.  One
-    // B200, in us by CTAs per tile: [1, 8192] x [8192, 8192]^T (64 tiles) 37.8, 28.5 with two, 25.2 with four, 30.7 with eight; [32, 4096] x [4096,
-    // 4096]^T (32 tiles) 21.0, 13.6, 9.8, 9.2.
-    // fp32 kernels fill an SM: what gives the fewest K blocks one after the other, a wave of clusters costing about kWave of them beside its own (launch,
-    // first loads, joining the sums).  Clusters that do not all fit at once are worth less than smaller ones that do: [256, 2048] x [1000, 2048]^T
-    // has 16 tiles, of which the GPU holds 15 as clusters of eight, and takes 30 us that way and 20 as clusters of four.
-    constexpr int64_t kWave = 6;
-    int split = 1;
-    if (size == 2) {
-        while (split < 8 && tiles * split * 2 <= 2 * tc::sm_count() && split * 2 <= args.k_blocks) split *= 2;
-    } else {
-        int64_t best = INT64_MAX;
-        for (int c = 1; c <= 8 && c <= args.k_blocks; ++c) {
-            const int64_t slots = cluster_slots(kernel, c, threads, smem, st, dev);
-            const int64_t cost = (tiles + slots - 1) / slots * ((args.k_blocks + c - 1) / c + kWave);
-            if (cost < best) {
-                best = cost;
-                split = c;
-            }
-        }
-    }
     if (tiles * split >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "Linear: too many tiles");
     CHXQ_CUDA(launch_pdl_cluster(split, kernel, dim3((unsigned)(tiles * split)), threads, smem, s, tmW, tmX, args, split, (int)x_tiles));
     count_launch(1);
@@ -154,14 +133,51 @@ int launch_tile(F* kernel, int bn, int threads, int smem, KernelState& st, const
 template <typename T, int BN, int STAGES>
 int launch_tile_16(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
     static KernelState state = {};
-    return launch_tile(lin::linear_tile_kernel<T, BN, STAGES>, BN, 256, lin::TileConfig<BN, STAGES>::kSmem, state, q, op, args, 2, s);
+    int dev = 0;
+    const int rc = current_device(&dev);
+    if (rc != CHXQ_OK) return rc;
+    // An SM holds two CTAs: the sharing CTAs are doubled as long as there are no more of them than that and each has a K block.  One B200, in us by
+    // CTAs per tile: [1, 8192] x [8192, 8192]^T (64 tiles) 37.8, 28.5 with two, 25.2 with four, 30.7 with eight; [32, 4096] x [4096, 4096]^T (32 tiles)
+    // 21.0, 13.6, 9.8, 9.2.
+    const int64_t tiles = ((q.M + BN - 1) / BN) * ((q.O + 127) / 128);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * tc::sm_count() && split * 2 <= args.k_blocks) split *= 2;
+    return launch_tile(lin::linear_tile_kernel<T, BN, STAGES>, BN, split, 256, lin::TileConfig<BN, STAGES>::kSmem, state, dev, q, op, args, 2, s);
 }
 
+// fp32 kernels fill an SM.
 template <int BN, int STAGES>
-int launch_tile_32(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
-    static KernelState state = {};
-    return launch_tile(lin::linear_tile_f32_kernel<BN, STAGES>, BN, 640, lin::TileF32Config<BN, STAGES>::kSmem, state, q, op, args, 4, s);
-}
+struct TileF32 {
+    using Cfg = lin::TileF32Config<BN, STAGES>;
+    int dev, split = 1, rc;
+    int64_t cost = INT64_MAX;
+
+    static KernelState& state() {
+        static KernelState st = {};
+        return st;
+    }
+    // How many CTAs share a tile: what is estimated to take the least time, in 0.01 us from one B200: 85 for a K block of a tile of 128 rows of x and 600
+    // for a wave of clusters beside that (launch, first loads, joining the sums), 72 and 400 up to 64 rows.  Clusters that do not all fit at once are
+    // worth less than smaller ones that do: [256, 2048] x [1000, 2048]^T has 16 tiles of 128 rows, of which the GPU holds 15 as clusters of eight, and
+    // takes 30 us that way and 18 as clusters of four.
+    TileF32(const chxq_linear_params& q, const lin::TcArgs& args, int device) : dev(device) {
+        rc = set_smem(lin::linear_tile_f32_kernel<BN, STAGES>, Cfg::kSmem, state(), dev);  // (the answers below ask for it)
+        if (rc != CHXQ_OK) return;
+        const int64_t tiles = ((q.M + BN - 1) / BN) * ((q.O + 127) / 128), block = BN == 128 ? 85 : 72, wave = BN == 128 ? 600 : 400;
+        for (int c = 1; c <= 8 && c <= args.k_blocks; ++c) {
+            const int64_t slots = cluster_slots(lin::linear_tile_f32_kernel<BN, STAGES>, c, 640, Cfg::kSmem, state(), dev);
+            const int64_t of = (tiles + slots - 1) / slots * ((args.k_blocks + c - 1) / c * block + wave);
+            if (of < cost) {
+                cost = of;
+                split = c;
+            }
+        }
+    }
+    int launch(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) const {
+        if (rc != CHXQ_OK) return rc;
+        return launch_tile(lin::linear_tile_f32_kernel<BN, STAGES>, BN, split, 640, Cfg::kSmem, state(), dev, q, op, args, 4, s);
+    }
+};
 
 template <typename T>
 int launch_pair(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
@@ -213,10 +229,17 @@ int launch_tc(const chxq_linear_params& q, const Operands& op, const lin::TcArgs
 
 template <>
 int launch_tc<float>(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
-    if (q.M <= 16) return launch_tile_32<16, 6>(q, op, args, s);
-    if (q.M <= 32) return launch_tile_32<32, 6>(q, op, args, s);
-    if (q.M <= 64) return launch_tile_32<64, 6>(q, op, args, s);
-    return launch_tile_32<128, 4>(q, op, args, s);
+    int dev = 0;
+    const int rc = current_device(&dev);
+    if (rc != CHXQ_OK) return rc;
+    if (q.M <= 16) return TileF32<16, 6>(q, args, dev).launch(q, op, args, s);
+    if (q.M <= 32) return TileF32<32, 6>(q, args, dev).launch(q, op, args, s);
+    const TileF32<64, 6> narrow(q, args, dev);
+    if (q.M <= 64) return narrow.launch(q, op, args, s);
+    // Few K blocks in few tiles: narrow ones, of which a wave is over sooner.  In us with 64 and 128 rows: [200, 200] x [200, 200]^T 7.7 and 9.8, [777, 555] x
+    // [1333, 555]^T 22.2 and 26.5, [600, 600] x [600, 600]^T 13.2 and 12.6, [1000, 1000] x [1000, 1000]^T 27.5 and 20.4, [813, 864] x [2662, 864]^T 51 and 34.
+    const TileF32<128, 4> wide(q, args, dev);
+    return narrow.cost < wide.cost ? narrow.launch(q, op, args, s) : wide.launch(q, op, args, s);
 }
 
 // A few rows of fp32.  No alignment is asked for: rows off 16-byte boundaries are read value by value ([1, 2147] x [2999, 2147]^T: 8 us, and 27 with copies in
