@@ -27,8 +27,10 @@ __global__ void __launch_bounds__(256) linear_empty_kernel(int64_t M, int64_t O,
 bool rows16(const void* p, int64_t ld, int64_t rows, int size) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || ld * size % 16 == 0);
 }
-int64_t pitch16(int64_t K, int size) {
-    const int per = 16 / size;
+// The rows of such a copy start on 128-byte lines: of others a row of a tile takes two ([2656, 5781] x [416, 5781]^T fp16: 43.7 us, and 56.7 with rows on
+// 16-byte boundaries).
+int64_t line_pitch(int64_t K, int size) {
+    const int per = 128 / size;
     return (K + per - 1) / per * per;
 }
 size_t align256(size_t v) {
@@ -287,8 +289,8 @@ extern "C" size_t chxq_linear_workspace(const chxq_linear_params* p) {
     if (!p || !is_float_type(p->dtype) || p->K <= 0 || p->M <= 0 || p->O <= 0 || few_rows(*p)) return 0;
     const int size = float_size(p->dtype);
     size_t n = 0;
-    if (!rows16(p->x, p->ldx, p->M, size)) n += align256((size_t)(p->M * pitch16(p->K, size)) * size);
-    if (!rows16(p->w, p->ldw, p->O, size)) n += align256((size_t)(p->O * pitch16(p->K, size)) * size);
+    if (!rows16(p->x, p->ldx, p->M, size)) n += align256((size_t)(p->M * line_pitch(p->K, size)) * size);
+    if (!rows16(p->w, p->ldw, p->O, size)) n += align256((size_t)(p->O * line_pitch(p->K, size)) * size);
     return n;
 }
 
@@ -315,7 +317,7 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     const int size = float_size(p->dtype);
     Operands op = {p->x, p->ldx, p->w, p->ldw};
     if (need) {
-        const int64_t pitch = pitch16(p->K, size);
+        const int64_t pitch = line_pitch(p->K, size);
         CopyJob jx = {p->x, p->ldx, 0, nullptr}, jw = {p->w, p->ldw, 0, nullptr};
         uint8_t* ws = static_cast<uint8_t*>(workspace);
         if (!rows16(p->x, p->ldx, p->M, size)) {
