@@ -438,7 +438,7 @@ def fuse_linear(program, epilogue=True):
                     act, u = take_activation(v)
                     if u:
                         first, chain, v = True, chain + u, insts[u[-1]].outputs[0]
-        name = i.inputs[1] + "@rows"
+        name = i.inputs[1] + ("@rows" if trans else "@columns")  # (a square matrix may be read both ways)
         added[name] = np.ascontiguousarray(w if trans else w.T)
         dropped.add(i.inputs[1])
         taken.update(chain)
@@ -957,7 +957,10 @@ class Executor:
         elif op == "LayerNormalization":
             if int(a.get("stash_type", 1)) != 1:
                 raise NotImplementedError("LayerNormalization: stash_type must be 1 (statistics in 32 bits)")
-            y = ops.LayerNormalization(x[0], x[1], x[2] if has(2) else None, axis=a.get("axis", -1), epsilon=a.get("epsilon", 1e-5), stats=len(inst.outputs) > 1)
+            shape = tuple(x[0].shape[a.get("axis", -1):])
+            scale, bias = (v if v is None or tuple(v.shape) == shape else v.broadcast_to((1,) * (v.dim() - len(shape)) + shape).reshape(shape)
+                           for v in (x[1], x[2] if has(2) else None))  # (they may broadcast)
+            y = ops.LayerNormalization(x[0], scale, bias, axis=a.get("axis", -1), epsilon=a.get("epsilon", 1e-5), stats=len(inst.outputs) > 1)
             for name, v in zip(inst.outputs, y if len(inst.outputs) > 1 else (y,)):
                 env[name] = v
         elif op == "LayerNormalizationGrad":

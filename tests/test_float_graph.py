@@ -92,6 +92,20 @@ def test_sixteen_bit_gemm_and_quantized_graphs(mods):
     assert [i.op for i in run_onnx.compile_model(model, quantize=True).insts][-2:] == ["Mul", "Add"]
 
 
+def test_one_matrix_read_both_ways(mods):
+    onnx_io, run_onnx = mods
+    rng = np.random.default_rng(1)
+    w = rng.standard_normal((4, 4)).astype(np.float16)
+    model = onnx_io.Model([onnx_io.Node("MatMul", ["x", "w"], ["p"], {}), onnx_io.Node("Gemm", ["p", "w"], ["q"], {"transB": 1}), onnx_io.Node("MatMul", ["q", "w"], ["y"], {})],
+                          {"w": w}, ["x"], ["y"])
+    prog = run_onnx.compile_model(model)
+    assert [i.op for i in prog.insts] == ["Linear"] * 3
+    for i, want in zip(prog.insts, (w.T, w, w.T)):
+        assert np.array_equal(prog.constants[i.inputs[1]], want)
+    out = run_onnx.program_to_onnx(prog)
+    assert [repr(n) for n in out.nodes] == [repr(n) for n in model.nodes] and np.array_equal(out.initializers["w"], w)
+
+
 def test_types_of_the_new_nodes(mods):
     onnx_io, run_onnx = mods
     nodes = [("LayerNormalization", ["x", "s4", "b4"], ["n", "mean", "inv"], {"axis": -1}), ("TokenLogProbs", ["n", "tok"], ["lp", "ent", "lse", "tl", "tt"], {"num_top": 2}),

@@ -119,6 +119,19 @@ def test_adds_that_broadcast(mods):
             _check(y.cpu(), want, 16 * E32 * mag + EF, (xs, rs))
 
 
+def test_scale_and_bias_that_broadcast(mods):
+    onnx_io, ops, run_onnx = mods
+    rng = np.random.default_rng(6)
+    x, r = rng.standard_normal((3, 5, 8)).astype(np.float32), lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    for axis, ss, bs in ((-1, (8,), (1, 1, 8)), (1, (8,), (5, 1)), (1, (1, 5, 8), (1,)), (2, (1, 8), ())):
+        s, b = r(*ss), r(*bs)
+        model = onnx_io.Model([onnx_io.Node("LayerNormalization", ["x", "s", "b"], ["y"], {"axis": axis})], {"s": s, "b": b}, ["x"], ["y"])
+        (_, y), = run_onnx.Executor(run_onnx.compile_model(model), "cuda:0").run({"x": x})
+        shape = x.shape[axis:]
+        full = [torch.from_numpy(np.broadcast_to(v.reshape(v.shape[max(0, v.ndim - len(shape)):]), shape).copy()).cuda() for v in (s, b)]
+        assert torch.equal(y, ops.LayerNormalization(torch.from_numpy(x).cuda(), full[0], full[1], axis=axis))
+
+
 def test_gradient_nodes_run_on_the_operators(mods):
     onnx_io, ops, run_onnx = mods
     rng = np.random.default_rng(4)

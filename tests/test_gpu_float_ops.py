@@ -135,6 +135,19 @@ def test_linear_offset_addresses_and_other_strides(ops, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_linear_of_a_vector(ops, dev, dtype):
+    g = torch.Generator(device=dev).manual_seed(8)
+    x, w, r = (torch.randn(s, device=dev, generator=g).to(dtype) for s in ((70,), (33, 70), (33,)))
+    want, bound = _linear64(x[None], w, None, "Tanh", r[None], True)
+    y = ops.Linear(x, w, activation="Tanh", residual=r, residual_first=True)
+    assert y.shape == (33,)
+    _check(y[None], want, bound)
+    wide = w[:1].expand(33, 70)  # rows that overlap
+    want, bound = _linear64(x[None], wide, None, None, r[None], False)
+    _check(ops.Linear(x, wide, residual=r)[None], want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_linear_without_sums_or_outputs(ops, dev, dtype):
     z = lambda *s: torch.zeros(s, dtype=dtype, device=dev)  # noqa: E731
     assert ops.Linear(z(0, 8), z(5, 8), activation="Relu").shape == (0, 5)
@@ -615,3 +628,36 @@ def test_a_block_captured_and_replayed_beside_another_stream(ops, dev):
         torch.cuda.current_stream().wait_stream(side)
         assert all(torch.equal(a, b) for a, b in zip(got, w)) and all(torch.equal(a, b) for a, b in zip(other, want_new))
     ops.device_status()
+
+
+def test_offsets_past_32_bits(ops, dev):
+    """More than 2^31 values in the operands and results: the last rows are those of a small call."""
+    def ends(full, part, rows):
+        return torch.equal(full[-rows:], part)
+
+    g = torch.Generator(device=dev).manual_seed(3)
+    x, w, r = torch.randn((70001, 16), device=dev, generator=g).bfloat16(), torch.randn((32768, 16), device=dev, generator=g).bfloat16(), None
+    y = ops.Linear(x, w, activation="Relu")  # 2.3e9 outputs
+    want, bound = _linear64(x[-200:], w, None, "Relu", r, False)
+    _check(y[-200:], want, bound)
+    del y
+    x = torch.empty((131100, 16411), dtype=torch.bfloat16, device=dev)  # 2.15e9
+    part = torch.randn((300, 16411), device=dev, generator=g).bfloat16()
+    x[:], x[-300:] = 1.0, part
+    s = torch.randn(16411, device=dev, generator=g)
+    y, mean, inv = ops.LayerNormalization(x, s, stats=True)
+    py, pm, pi = ops.LayerNormalization(part, s, stats=True)
+    assert torch.equal(mean[-300:], pm) and torch.equal(inv[-300:], pi) and torch.equal(y[-300:], py)
+    dx = ops.LayerNormalizationGrad(x, x, s, mean, inv)[0]
+    assert ends(dx[-290:-10], ops.LayerNormalizationGrad(part, part, s, pm, pi)[0][10:-10], 280)
+    del dx, y
+    tok = torch.randint(0, 16411, (131100,), device=dev, generator=g)
+    lp, ent, lse, tl, tt = ops.TokenLogProbs(x, tok, 3)
+    a = ops.TokenLogProbs(part, tok[-300:], 3)
+    ref = torch.log_softmax(part.double(), dim=1).gather(1, tok[-300:, None])[:, 0]
+    sums = (16411 + 16) * E32  # of a row, and its logarithm
+    assert ((lp[-300:].double() - ref).abs() <= sums + 4 * E32 * ref.abs()).all() and torch.equal(tt[-300:], a[4])
+    assert ((lse[-300:] - a[2]).abs() <= 2 * sums + 2 * E32 * a[2].abs()).all()
+    one = torch.ones(131100, device=dev)
+    d = ops.TokenLogProbsGrad(one, None, x, tok, lse)
+    assert ends(d, ops.TokenLogProbsGrad(one[-300:], None, part, tok[-300:], lse[-300:]), 300)
