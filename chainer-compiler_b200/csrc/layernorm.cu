@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) layernorm_kernel(const T* 
     float is = rsqrtf(var);
     is = is * fmaf(-0.5f * var * is, is, 1.5f);  // one Newton step on the approximation, which is good to 2^-22
     if (var == 0.f) is = INFINITY;               // (epsilon 0 and a constant row)
+    if (var == INFINITY) is = 0.f;               // (squares past the range of 32 bits; the step would make NaN of it)
     const f32x2 is2 = make_x2(is, is);
     if (!live) return;
 #pragma unroll

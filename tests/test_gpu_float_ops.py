@@ -251,6 +251,19 @@ def test_layernorm_axes_strides_and_constant_rows(ops, dev, dtype):
     assert torch.isnan(y[1]).all() and not torch.isnan(y[[0, 2]]).any()
 
 
+@pytest.mark.parametrize("d", [64, 1000, 40000])
+def test_layernorm_of_rows_whose_squares_overflow(ops, dev, d):
+    """A variance that is infinite in 32 bits gives an inverse deviation of zero, not NaN, and leaves the other rows alone."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn((3, d), device=dev, generator=torch.Generator(device=dev).manual_seed(4)).to(dtype)
+        x[1] = 1e25
+        x[1, ::2] = -1e25
+        s, b = torch.ones(d, device=dev), torch.full((d,), 0.5, device=dev)
+        y, mean, inv = ops.LayerNormalization(x, s, b, stats=True)
+        assert float(inv[1]) == 0 and float(mean[1].abs()) <= 1e25 and torch.equal(y[1], torch.full_like(y[1], 0.5))
+        assert torch.equal(y[[0, 2]], ops.LayerNormalization(x[[0, 2]], s, b))
+
+
 def _grad64(dy, x, scale, mean, inv):
     dy, xh = dy.double(), (x.double() - mean.double()) * inv.double()
     gd = dy * scale.double()
