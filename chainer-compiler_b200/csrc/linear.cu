@@ -2,7 +2,7 @@
 // sums in 32 bits, one rounding at the end.
 //
 // Three kernels: CTA pairs with 256 x 256 blocks (linear_pair.cuh) for large 16-bit products, clusters that share a tile's K (linear_tile.cuh) for
-// few rows of x, for products in between and for fp32, and threads side by side along K for a few rows of fp32 (linear_rows.cuh).
+// few rows of x, for products in between and for fp32, and threads side by side along K for few rows or outputs (linear_rows.cuh).
 #include <algorithm>
 #include <atomic>
 
@@ -244,26 +244,33 @@ int launch_tc<float>(const chxq_linear_params& q, const Operands& op, const lin:
     return narrow.cost < wide.cost ? narrow.launch(q, op, args, s) : wide.launch(q, op, args, s);
 }
 
-// A few rows of fp32.  No alignment is asked for: rows off 16-byte boundaries are read value by value ([1, 2147] x [2999, 2147]^T: 8 us, and 27 with copies in
-// front of tiles).
-template <int MR>
+// Few rows or outputs.  No alignment is asked for: rows off 16-byte boundaries are read value by value ([1, 2147] x [2999, 2147]^T fp32: 8 us, and 27 with copies
+// in front of tiles).
+template <typename T, int MR>
 int launch_rows(const chxq_linear_params& q, const LinearEpilogue& e, cudaStream_t s) {
-    constexpr int R = 4;
-    const bool vec = rows16(q.x, q.ldx, q.M, 4) && rows16(q.w, q.ldw, q.O, 4);
-    const int64_t blocks = (q.O + R - 1) / R, pieces = vec ? q.K / 4 : q.K;
+    constexpr int R = 4, VEC = 16 / (int)sizeof(T);
+    const bool vec = rows16(q.x, q.ldx, q.M, sizeof(T)) && rows16(q.w, q.ldw, q.O, sizeof(T));
+    const int64_t blocks = (q.O + R - 1) / R, pieces = vec ? q.K / VEC : q.K;
     const int threads = (int)std::min<int64_t>(blocks <= tc::sm_count() ? 512 : 256, std::max<int64_t>(32, (pieces + 31) / 32 * 32));
-    auto* kernel = vec ? lin::linear_rows_kernel<MR, R, 4, MR <= 2 ? 4 : (MR == 4 ? 2 : 1)> : lin::linear_rows_kernel<MR, R, 1, MR <= 2 ? 8 : 4>;
-    CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)blocks, (unsigned)((q.M + MR - 1) / MR)), threads, 0, s, static_cast<const float*>(q.x), q.ldx, static_cast<const float*>(q.w), q.ldw, (int)q.M, (int)q.O,
-                         (int)q.K, e));
+    auto* kernel = vec ? lin::linear_rows_kernel<T, MR, R, VEC, MR <= 2 ? 4 : (MR == 4 ? 2 : 1)> : lin::linear_rows_kernel<T, MR, R, 1, MR <= 2 ? 8 : 4>;
+    CHXQ_CUDA(launch_pdl(kernel, dim3((unsigned)blocks, (unsigned)((q.M + MR - 1) / MR)), threads, 0, s, static_cast<const T*>(q.x), q.ldx, static_cast<const T*>(q.w), q.ldw,
+                         (int)q.M, (int)q.O, (int)q.K, e));
     count_launch(1);
     return CHXQ_OK;
 }
 
-// Up to eight rows, one block for all of them; up to sixteen, two blocks for eight each, where the blocks run in two waves (two are on an SM at once):
-// [16, 2048] x [1000, 2048]^T 6.5 us against 11.6 in tiles, [16, 1024] x [4096, 1024]^T 15.2 against 11.7.
+// Which products they take.  Up to eight rows of fp32, and more of any type in blocks of eight where those run in two waves (two are on an SM at once).
+// 16-bit tiles read the weights as fast and convert none: they are left what takes longer than the start of a tile, about 2 us + (0.32 + 0.047 M) us per
+// 2^20 weights here against 4.6 + 0.305.  Rows off 16-byte boundaries, read value by value here, tiles copy first.  In us here and in tiles: [1, 1024] x
+// [4096, 1024]^T bf16 3.8 and 6.2, [8, 1024] x [4096, 1024]^T 5.4 and 6.3, [8, 4096] x [4096, 4096]^T 13.4 and 8.3, [64, 2000] x [64, 2000]^T fp16 3.1 and
+// 6.8, [4, 1023] x [4096, 1023]^T fp16 9.1 and 11.2; fp32: [64, 8192] x [64, 8192]^T 5.4 and 27, [411, 2000] x [16, 2000]^T 5.4 and 11.8, [64, 2048] x [250,
+// 2048]^T 10.1 and 12.2.
 bool few_rows(const chxq_linear_params& q) {
-    if (q.dtype != CHXQ_FLOAT32 || q.M > lin::kRowsMost) return false;
-    return q.M <= 8 || (q.O + 3) / 4 * 2 <= 4 * tc::sm_count();
+    if (q.M > 8 && (q.O + 3) / 4 * ((q.M + 7) / 8) > 4 * tc::sm_count()) return false;
+    if (q.dtype == CHXQ_FLOAT32) return true;
+    const int64_t values = q.O * q.K;
+    if (rows16(q.x, q.ldx, q.M, 2) && rows16(q.w, q.ldw, q.O, 2)) return values * (1 + 3 * q.M) <= 110000000;
+    return q.M <= 4 || values <= 4200000;
 }
 
 }  // namespace
@@ -310,9 +317,12 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
             return CHXQ_OK;
         });
     if (few_rows(*p)) {
-        if (p->M == 1) return launch_rows<1>(*p, e, s);
-        if (p->M == 2) return launch_rows<2>(*p, e, s);
-        return p->M <= 4 ? launch_rows<4>(*p, e, s) : launch_rows<8>(*p, e, s);
+        return with_float_type(p->dtype, [&](auto t) {
+            using T = decltype(t);
+            if (p->M == 1) return launch_rows<T, 1>(*p, e, s);
+            if (p->M == 2) return launch_rows<T, 2>(*p, e, s);
+            return p->M <= 4 ? launch_rows<T, 4>(*p, e, s) : launch_rows<T, 8>(*p, e, s);
+        });
     }
     const int size = float_size(p->dtype);
     Operands op = {p->x, p->ldx, p->w, p->ldw};

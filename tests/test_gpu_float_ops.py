@@ -68,12 +68,14 @@ def _check_linear(ops, dev, m, k, o, dtype, act, residual, bias=True, bias32=Fal
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("residual", [None, "last", "first"])
-def test_linear_epilogues(ops, dev, dtype, act, residual):
-    _check_linear(ops, dev, 37, 96, 72, dtype, act, residual, bias32=residual is None)
+@pytest.mark.parametrize("m,k,o", [(37, 96, 72), (20, 96, 2500), (140, 96, 600), (1100, 64, 2048)])  # one for each kernel
+def test_linear_epilogues(ops, dev, dtype, act, residual, m, k, o):
+    _check_linear(ops, dev, m, k, o, dtype, act, residual, bias32=residual is None)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,k,o", [(1, 1, 1), (1, 0, 5), (3, 8, 1), (1, 512, 4096), (2, 2048, 1000), (16, 64, 16), (17, 200, 33), (33, 1283, 129), (128, 128, 128), (129, 72, 257),
+                                   (3, 4096, 5000), (9, 200, 3001), (20, 333, 2500), (40, 1283, 1999), (64, 8, 5000), (61, 8192, 1300),
                                    (256, 2048, 1000), (300, 33, 511), (509, 1283, 997), (1024, 512, 768), (777, 4096, 640), (2500, 264, 1500)])
 def test_linear_extents(ops, dev, dtype, m, k, o):
     _check_linear(ops, dev, m, k, o, dtype, "Gelu", "last" if o % 2 else "first", bias=m != 3)
@@ -86,10 +88,11 @@ def test_linear_rows_of_wider_buffers(ops, dev, dtype, pitch, m):
     _check_linear(ops, dev, m, 320, 264, dtype, "Swish", "last", pitch=pitch)
 
 
-@pytest.mark.parametrize("m", list(range(1, 10)) + [16])
-@pytest.mark.parametrize("k,o,pitch", [(4100, 5, 0), (1023, 131, 0), (70, 2050, 1), (3, 64, 4), (6948, 26, 0), (2047, 700, 5)])
-def test_linear_few_rows_of_fp32(ops, dev, m, k, o, pitch):
-    _check_linear(ops, dev, m, k, o, torch.float32, "Tanh", "first" if m % 2 else "last", pitch=pitch)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", list(range(1, 10)) + [16, 25, 400])
+@pytest.mark.parametrize("k,o,pitch", [(4100, 5, 0), (1023, 131, 0), (70, 2050, 1), (3, 64, 4), (6948, 26, 0), (2047, 700, 5), (64, 30, 8)])
+def test_linear_few_outputs(ops, dev, dtype, m, k, o, pitch):
+    _check_linear(ops, dev, m, k, o, dtype, "Tanh", "first" if m % 2 else "last", pitch=pitch)
 
 
 @pytest.mark.parametrize("m,k,o", [(2048, 64, 2000), (1900, 17, 2100), (349, 500, 3125), (1024, 33, 1000), (300, 40, 5000), (65, 300, 20000), (2200000, 3, 2)])
@@ -159,13 +162,13 @@ def test_linear_without_sums_or_outputs(ops, dev, dtype):
 def test_linear_special_values(ops, dev):
     """NaN and infinities travel as the formula has them; an activation of a large negative value is zero, not NaN."""
     for dtype in TYPES:
-        for m in (1, 200):
+        for m, o in ((1, 16), (200, 16), (20, 2500), (200, 1100), (1100, 2048)):
             x = torch.zeros((m, 64), dtype=dtype, device=dev)
-            w = torch.zeros((16, 64), dtype=dtype, device=dev)
+            w = torch.zeros((o, 64), dtype=dtype, device=dev)
             w[:, 0] = 1
             x[:, 0] = torch.tensor([float("nan"), float("inf"), -300.0, 300.0], dtype=dtype, device=dev)[torch.arange(m, device=dev) % 4]
             for act in ACTS:
-                y = ops.Linear(x, w, activation=act, residual=torch.zeros((m, 16), dtype=dtype, device=dev)).float()
+                y = ops.Linear(x, w, activation=act, residual=torch.zeros((m, o), dtype=dtype, device=dev)).float()
                 assert torch.isnan(y[0]).all(), act
                 if m > 1:
                     assert torch.equal(y[1], torch.full_like(y[1], 1.0 if act in ("Sigmoid", "Tanh") else float("inf"))), act
