@@ -24,6 +24,8 @@ DTYPE_BY_NAME = {"float16": FLOAT16, "float32": FLOAT32, "float64": FLOAT64}
 # activations of Linear's epilogue
 ACTIVATIONS = {None: 0, "Relu": 1, "Gelu": 2, "GeluTanh": 3, "Swish": 4, "Sigmoid": 5, "Tanh": 6}
 MAX_TOP = 32
+# kernels of chxq_linear
+LINEAR_NO_PRODUCT, LINEAR_ROWS, LINEAR_TILES, LINEAR_PAIRS, LINEAR_TILES_F32 = range(5)
 EW_OPS = {"Identity": 0, "Tanh": 1, "Exp": 2, "Sigmoid": 3, "Add": 4, "Sub": 5, "Mul": 6, "Div": 7, "Constant": 8}
 
 
@@ -137,6 +139,7 @@ SIGNATURES = {
     "chxq_conv_dev_workspace": (_sz, [_c.POINTER(ConvGeom)]),
     "chxq_conv_integer_dev_ws": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
     "chxq_linear_workspace": (_sz, [_c.POINTER(LinearParams)]),
+    "chxq_linear_kernel": (_c.c_int, [_c.POINTER(LinearParams), _c.POINTER(_i32)]),
     "chxq_linear": (_c.c_int, [_c.POINTER(LinearParams), _vp, _sz, _vp]),
     "chxq_layernorm": (_c.c_int, [_vp, _i64, _i32, _vp, _vp, _i32, _i64, _i64, _f32, _vp, _vp, _vp, _vp]),
     "chxq_layernorm_grad_workspace": (_sz, [_i64, _i64]),

@@ -208,19 +208,27 @@ int launch_pair(const chxq_linear_params& q, const Operands& op, const lin::TcAr
     return CHXQ_OK;
 }
 
+int k_blocks_of(const chxq_linear_params& q) {  // of 128 bytes
+    return (int)((q.K * float_size(q.dtype) + 127) / 128);
+}
+
+// Pairs or single tiles (16-bit operands), in units of 0.01 us from one B200: a K block of a 256 x 256 block takes a pair 0.27 us and a launch 6 beside
+// that; a K block of a 128 x 128 tile takes an SM 0.27 us, too, and 0.3 at least where its CTA is alone.  [512, 4096] x [4096, 4096]^T: 25.3 us in
+// pairs, 22.5 in tiles; [1024, 4096] x [4096, 4096]^T: 27.0 and 35.7; [8192, 64] x [1024, 64]^T: 10.1 and 18.8.
+bool takes_pairs(const chxq_linear_params& q) {
+    if (q.M <= 128) return false;
+    const int64_t tiles128 = ((q.M + 127) / 128) * ((q.O + 127) / 128);
+    const int64_t sms = tc::sm_count(), blocks = ((q.M + 255) / 256) * ((q.O + 255) / 256), kb = k_blocks_of(q);
+    const int64_t pairs = (blocks + sms / 2 - 1) / (sms / 2) * kb * 27 + 600;
+    const int64_t share = std::min<int64_t>(8, std::max<int64_t>(1, 2 * sms / tiles128));
+    const int64_t tiles = std::max(tiles128 * kb * 27 / sms, (kb + share - 1) / share * 30) + 500 + tiles128 / (2 * sms) * 300;
+    return pairs <= tiles;
+}
+
 template <typename T>
 int launch_tc(const chxq_linear_params& q, const Operands& op, const lin::TcArgs& args, cudaStream_t s) {
+    if (takes_pairs(q)) return launch_pair<T>(q, op, args, s);
     const int64_t tiles128 = ((q.M + 127) / 128) * ((q.O + 127) / 128);
-    if (q.M > 128) {
-        // Pairs or single tiles, in units of 0.01 us from one B200: a K block of a 256 x 256 block takes a pair 0.27 us and a launch 6 beside that; a K
-        // block of a 128 x 128 tile takes an SM 0.27 us, too, and 0.3 at least where its CTA is alone.  [512, 4096] x [4096, 4096]^T: 25.3 us in
-        // pairs, 22.5 in tiles; [1024, 4096] x [4096, 4096]^T: 27.0 and 35.7; [8192, 64] x [1024, 64]^T: 10.1 and 18.8.
-        const int64_t sms = tc::sm_count(), blocks = ((q.M + 255) / 256) * ((q.O + 255) / 256), kb = args.k_blocks;
-        const int64_t pairs = (blocks + sms / 2 - 1) / (sms / 2) * kb * 27 + 600;
-        const int64_t share = std::min<int64_t>(8, std::max<int64_t>(1, 2 * sms / tiles128));
-        const int64_t tiles = std::max(tiles128 * kb * 27 / sms, (kb + share - 1) / share * 30) + 500 + tiles128 / (2 * sms) * 300;
-        if (pairs <= tiles) return launch_pair<T>(q, op, args, s);
-    }
     if (q.M <= 16) return launch_tile_16<T, 16, 6>(q, op, args, s);
     if (q.M <= 32) return launch_tile_16<T, 32, 5>(q, op, args, s);
     // Narrow tiles also where wide ones are so few that eight CTAs each do not fill the SMs twice: [256, 2048] x [1000, 2048]^T 9.1 against 10.5 us, [128,
@@ -301,6 +309,17 @@ extern "C" size_t chxq_linear_workspace(const chxq_linear_params* p) {
     return n;
 }
 
+extern "C" int chxq_linear_kernel(const chxq_linear_params* p, int32_t* kernel) {
+    CHXQ_CHECK_ARG(kernel != nullptr, "Linear: null pointer");
+    const int rc = check_linear(p);
+    if (rc != CHXQ_OK) return rc;
+    if (p->M == 0 || p->O == 0 || p->K == 0) *kernel = CHXQ_LINEAR_NO_PRODUCT;
+    else if (few_rows(*p)) *kernel = CHXQ_LINEAR_ROWS;
+    else if (p->dtype == CHXQ_FLOAT32) *kernel = CHXQ_LINEAR_TILES_F32;
+    else *kernel = takes_pairs(*p) ? CHXQ_LINEAR_PAIRS : CHXQ_LINEAR_TILES;
+    return CHXQ_OK;
+}
+
 extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_linear(p);
     if (rc != CHXQ_OK) return rc;
@@ -349,7 +368,7 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     lin::TcArgs a;
     a.M = (int)p->M;
     a.O = (int)p->O;
-    a.k_blocks = (int)((p->K * size + 127) / 128);
+    a.k_blocks = k_blocks_of(*p);
     a.idesc = lin::idesc_f16(p->dtype == CHXQ_BFLOAT16 ? lin::kBf16 : lin::kF16);  // (fp32 has its own)
     a.e = e;
     a.vec = rows16(p->y, p->ldy, p->M, size) && p->O * size % 16 == 0 && (!p->residual || rows16(p->residual, p->ldr, p->M, size));

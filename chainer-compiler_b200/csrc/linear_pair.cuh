@@ -199,8 +199,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     if (issuer) tma_store_wait_read<0>();
                     bar_sync(2 + group, 128);  // the staged tile is free
                     if (p.e.residual) {
-                        // rows off 16-byte boundaries: a warp copies its 32 rows, 64 values each
-                        const int r0 = (e & 3) * 32, n = min(32, p.M - m0 - r0);
+                        // rows off 16-byte boundaries: a warp copies the 32 rows that its own lanes read below and write their outputs to, 64 values each
+                        // (no other warp touches them before the group's barrier)
+                        const int r0 = quarter * 32, n = min(32, p.M - m0 - r0);
                         const T* src = static_cast<const T*>(p.e.residual) + (int64_t)(m0 + r0) * p.e.ldr + col + lane;
                         const bool in0 = col + lane < p.O, in1 = col + lane + 32 < p.O;
 #pragma unroll 8

@@ -7,6 +7,8 @@
 
 #include <stdint.h>
 
+#include "chxq.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -33,6 +35,13 @@ int chxq_tc_test_hooks(int64_t wait_limit_ns, int32_t skip_weight_load_kb);
  * (cudaOccupancyMaxActiveClusters): the kernel's grid is twice this, or smaller for small problems. */
 int chxq_tc_pair_slots(int32_t* slots);
 
+/* Which kernel chxq_linear runs for these parameters on the current device (one B200's numbers where there is none); nothing is launched. */
+#define CHXQ_LINEAR_NO_PRODUCT 0 /* no outputs, or no K */
+#define CHXQ_LINEAR_ROWS 1       /* few rows or outputs, fp32 pipes */
+#define CHXQ_LINEAR_TILES 2      /* 16-bit tiles, a cluster per tile */
+#define CHXQ_LINEAR_PAIRS 3      /* 16-bit blocks of 256 x 256 on CTA pairs */
+#define CHXQ_LINEAR_TILES_F32 4  /* fp32 tiles, split operands */
+int chxq_linear_kernel(const chxq_linear_params* p, int32_t* kernel);
 
 #ifdef __cplusplus
 }
