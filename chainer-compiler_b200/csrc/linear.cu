@@ -23,6 +23,10 @@ __global__ void __launch_bounds__(256) linear_empty_kernel(int64_t M, int64_t O,
 
 // ---- the tensor-core kernels ------------------------------------------------------------------------------------------------
 
+// Bytes of a row and rows of an operand for one launch of the tensor-core kernels, half of what TMA's 32-bit coordinates count: a tile past 2^31 is an
+// illegal instruction.
+constexpr int64_t kMostCoordinate = 1ll << 30;
+
 // TMA reads rows that start on 16-byte boundaries.  Operands whose rows do not are copied into such rows in front of the product.
 bool rows16(const void* p, int64_t ld, int64_t rows, int size) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows == 1 || ld * size % 16 == 0);
@@ -273,7 +277,9 @@ int launch_rows(const chxq_linear_params& q, const LinearEpilogue& e, cudaStream
 // [4096, 1024]^T bf16 3.8 and 6.2, [8, 1024] x [4096, 1024]^T 5.4 and 6.3, [8, 4096] x [4096, 4096]^T 13.4 and 8.3, [64, 2000] x [64, 2000]^T fp16 3.1 and
 // 6.8, [4, 1023] x [4096, 1023]^T fp16 9.1 and 11.2; fp32: [64, 8192] x [64, 8192]^T 5.4 and 27, [411, 2000] x [16, 2000]^T 5.4 and 11.8, [64, 2048] x [250,
 // 2048]^T 10.1 and 12.2.
+// And rows of more than 2^30 bytes, whatever their number: TMA counts a row's bytes in 32 signed bits.
 bool few_rows(const chxq_linear_params& q) {
+    if (q.K * float_size(q.dtype) > kMostCoordinate) return true;
     if (q.M > 8 && (q.O + 3) / 4 * ((q.M + 7) / 8) > 4 * tc::sm_count()) return false;
     if (q.dtype == CHXQ_FLOAT32) return true;
     const int64_t values = q.O * q.K;
@@ -324,6 +330,24 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     const int rc = check_linear(p);
     if (rc != CHXQ_OK) return rc;
     if (p->M == 0 || p->O == 0) return CHXQ_OK;
+    if (p->M > kMostCoordinate || p->O > kMostCoordinate) {  // (one workspace for all: each launch waits for the one before)
+        const int64_t size = float_size(p->dtype), bias_size = p->bias ? float_size(p->bias_dtype) : 0;
+        auto at = [](const void* base, int64_t bytes) { return base ? static_cast<const uint8_t*>(base) + bytes : nullptr; };
+        for (int64_t m = 0; m < p->M; m += kMostCoordinate)
+            for (int64_t o = 0; o < p->O; o += kMostCoordinate) {
+                chxq_linear_params q = *p;
+                q.M = std::min(kMostCoordinate, p->M - m);
+                q.O = std::min(kMostCoordinate, p->O - o);
+                q.x = at(p->x, m * p->ldx * size);
+                q.w = at(p->w, o * p->ldw * size);
+                q.bias = at(p->bias, o * bias_size);
+                q.residual = at(p->residual, (m * p->ldr + o) * size);
+                q.y = const_cast<uint8_t*>(at(p->y, (m * p->ldy + o) * size));
+                const int part = chxq_linear(&q, workspace, workspace_bytes, stream);
+                if (part != CHXQ_OK) return part;
+            }
+        return CHXQ_OK;
+    }
     const size_t need = chxq_linear_workspace(p);
     if (need && (!workspace || workspace_bytes < need)) return set_error(CHXQ_ERR_WORKSPACE, "Linear: needs %zu bytes of workspace", need);
     CHXQ_CHECK_ARG(need == 0 || (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "Linear: the workspace must be 256-byte aligned");

@@ -35,6 +35,17 @@ def test_the_other_kernels(pkg):
     assert route(pkg, 0, 8, 8) == route(pkg, 8, 0, 8) == route(pkg, 8, 8, 0) == _lib.LINEAR_NO_PRODUCT
 
 
+@pytest.mark.parametrize("dtype,size", [("float16", 2), ("bfloat16", 2), ("float32", 4)])
+def test_rows_whose_bytes_pass_the_coordinates_of_tma(pkg, dtype, size):
+    """(TMA's coordinates are 32 signed bits; the kernels that use it count bytes along a row.)"""
+    from chainer_compiler_b200 import _lib
+    for m, o in ((1, 1), (1, 2), (5, 1), (9, 3), (40, 40), (200, 700)):
+        for k in ((1 << 31) // size - 64, (1 << 31) // size + 8, (1 << 30) + 264):
+            assert route(pkg, m, k, o, dtype) == _lib.LINEAR_ROWS
+    if size == 2:
+        assert route(pkg, 1, 1 << 28, 8, dtype) == _lib.LINEAR_TILES
+
+
 def test_refusals(pkg):
     from chainer_compiler_b200 import _lib
     bad = -_lib.ERR_INVALID_ARGUMENT
