@@ -188,7 +188,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
             }
         }
         __syncwarp();
-        if (counts[warp] > kBuffer / 2) settle();
+        const bool many = counts[warp] > kBuffer / 2;
+        __syncwarp();  // (all lanes have read it before one of them adds to it again, so that they settle together or not at all)
+        if (many) settle();
     };
     auto grow = [&](float to) {  // a larger maximum
         const float d = max_nan(m - to, -1e4f), f = exp2_approx(d * kLog2e);  // (as in rescale; the sums are zero while m is -infinity)
