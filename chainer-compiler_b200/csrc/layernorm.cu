@@ -50,13 +50,13 @@ struct Place {
     __device__ __forceinline__ bool has(int i, int j) const { return (unsigned)(column(i) + j) < (unsigned)D; }
 
     // Piece i of the row at `row`; zero where the thread has none.  Rows of whole pieces: the first one is read instead, so that no branch parts the
-    // loads ([4096, 12000] fp32: 104 -> 70 us).  SHIFT: the last row's last piece may reach past the buffer and is read value by value.
-    __device__ __forceinline__ void load(const T* row, int i, bool last_row, Pack<T, VEC>& v) const {
+    // loads ([4096, 12000] fp32: 104 -> 70 us).  SHIFT: at the end of the buffer a row's last piece may reach past it and is read value by value.
+    __device__ __forceinline__ void load(const T* row, int i, bool end, Pack<T, VEC>& v) const {
         if constexpr (!SHIFT) {
             v.load(row + (any(i) ? column(i) : 0));
             if (!any(i)) v.zero();
         } else {
-            const bool tail = last_row && column(i) + VEC > D;
+            const bool tail = end && column(i) + VEC > D;
             v.zero();
             if (any(i) && !tail) v.load(row + column(i));
             if (tail)
@@ -66,8 +66,8 @@ struct Place {
         }
     }
     // The same for a row that is not looked at yet: nothing here waits for the load, so a piece that the thread does not have is left as it is.
-    __device__ __forceinline__ void load_ahead(const T* row, int i, bool last_row, Pack<T, VEC>& v) const {
-        const bool tail = SHIFT && last_row && column(i) + VEC > D;
+    __device__ __forceinline__ void load_ahead(const T* row, int i, bool end, Pack<T, VEC>& v) const {
+        const bool tail = SHIFT && end && column(i) + VEC > D;
         if (any(i) && !tail) v.load(row + column(i));
         if (tail) {
             v.zero();
@@ -114,6 +114,12 @@ struct Place {
         }
     }
 };
+
+// Whether pieces of row r may reach past the end of the buffer: the last row's, and of rows shorter than a piece any of the last ones'.
+template <int VEC>
+__device__ __forceinline__ bool at_end(int64_t r, int64_t rows, int D) {
+    return r >= rows - (D < VEC ? VEC : 1);
+}
 
 // Sums over a group of G <= 32 threads, the same for all of them.
 template <int N>
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) layernorm_kernel(const T* 
         Pack<T, VEC> q[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (live) at.load(xr, i, r == rows - 1, q[i]);
+            if (live) at.load(xr, i, at_end<VEC>(r, rows, D), q[i]);
             else q[i].zero();
         }
 #pragma unroll
@@ -305,8 +311,8 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
     if (r < rows) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            at.load_ahead(px, i, r == rows - 1, nx[i]);
-            at.load_ahead(pd, i, r == rows - 1, nd[i]);
+            at.load_ahead(px, i, at_end<VEC>(r, rows, D), nx[i]);
+            at.load_ahead(pd, i, at_end<VEC>(r, rows, D), nd[i]);
         }
         nm = mean[r];
         ns = inv[r];
@@ -333,8 +339,8 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
         if (r + step < rows) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                at.load_ahead(px, i, r + step == rows - 1, nx[i]);
-                at.load_ahead(pd, i, r + step == rows - 1, nd[i]);
+                at.load_ahead(px, i, at_end<VEC>(r + step, rows, D), nx[i]);
+                at.load_ahead(pd, i, at_end<VEC>(r + step, rows, D), nd[i]);
             }
             nm = mean[r + step];
             ns = inv[r + step];
