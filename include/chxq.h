@@ -336,7 +336,7 @@ int chxq_maxpool_u8_nhwc(const uint8_t* x, int32_t N, int32_t H, int32_t W, int3
                          int32_t Wo, uint8_t* y, void* stream);
 /* Global AveragePool (pooling.cc:62-75) fused with DequantizeLinear: y[n,c] = mean((q - zp)) * scale. */
 int chxq_global_avgpool_dq_nhwc(const uint8_t* x, int32_t N, int32_t HW, int32_t C, float scale, int32_t zp, float* y, void* stream);
-/* Linear / Gemm (runtime/ops/connection.cc:12-15): y[n,o] = sum_k x[n,k] w[o,k] + b[o], fp32. */
+/* Linear / Gemm (runtime/ops/connection.cc:12-15): y[n,o] = sum_k x[n,k] w[o,k] + b[o], fp32; K < 2^31 - 1024. */
 int chxq_linear_f32(const float* x, const float* w, const float* b, int32_t N, int32_t K, int32_t O, float* y, void* stream);
 /* DequantizeLinear, DequantizeLinear, Add, (Relu), QuantizeLinear of two u8 maps in one pass. */
 int chxq_qadd_u8(const uint8_t* a, float a_scale, int32_t a_zp, const uint8_t* b, float b_scale, int32_t b_zp, int64_t n, float y_scale,
