@@ -225,19 +225,20 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant_
 
 // ---- fp32 operands ---------------------------------------------------------------------------------------------------------
 //
-// The tensor cores multiply tf32, eleven significant bits.  A value is split as a = h + l with h = tf32(a) and l = tf32(a - h), rounded to nearest, and the
-// product taken as h h' + h l' + l h': what is left out is below 2^-21 |a a'|, the rounding of an fp32 product in a sum of a few.
+// The tensor cores multiply tf32, eleven significant bits.  A value is split as a = h + l with h = tf32(a) and l = tf32(a - h), rounded to nearest, 22 bits in
+// all, and the product taken as h h' + h l' + l h': what is left out is below 2^-21 |a a'|, the rounding of an fp32 product in a sum of a few.  (Sums of fewer
+// than 32 terms are therefore further off than a chain of fp32 products, 9.8e-8 against 4.2e-8 for K = 4.)
 // The sums: h h' goes through TMEM in chains of kChain K blocks (at most 16 instructions, whose additions the tensor core may truncate), each then
 // added in registers; the two small products have an accumulator of their own, 2^-11 in size, for the whole of K.  [2048, 2048] x [2048, 2048]^T:
 // 3.5e-7 off the sums in 64 bits (root mean square, relative); chains of eight 6.4e-7 for 2% less time, of two 2.2e-7 for 5% more; an fp32
 // product 8.1e-7.
 // The operands: w is split into tensor memory, two stages of h and l, x in place in shared memory with l beside it.  (Both in shared memory: 192 KB of
-// traffic a K block instead of 112, 140 us for 2048^3 where this takes 109.)  h and l of x are neighbours, so that one instruction of 2 BN columns
+// traffic a K block instead of 112, 140 us for 2048^3 where this takes 112.)  h and l of x are neighbours, so that one instruction of 2 BN columns
 // takes h of w times both: h h' into the chain's accumulator and h l' into the small products'.  Those lie between the accumulators of even and of odd
 // chains, and x's halves change places with the chain.  Since the instruction adds to both or to none, a chain starts from zeros that are written.
 // Roles as above, with 640 threads: warps 0 and 2 load, warp 1 issues, warps 4-19 split, in two groups that take the K blocks by turns, drain the chains and
 // run the epilogue.
-// Bound: a K block of 128 x 128 takes 0.8 us where the tensor pipe needs 0.41: the splitting (some twenty-three instructions per sixteen bytes) and the
+// Bound: a K block of 128 x 128 takes 0.8 us where the tensor pipe needs 0.41: the splitting (some twenty instructions per sixteen bytes) and the
 // issuing thread (eight products and a commit of 75 to 90 cycles each beside busy warps).
 template <int BN, int STAGES>
 struct TileF32Config {
@@ -252,31 +253,36 @@ struct TileF32Config {
     static_assert(kSmem <= 227 * 1024, "shared memory over the per-CTA limit");
 };
 
-// v = h + l + a rest below 2^-22 |v|, by integer rounding (the conversion instruction runs at a sixteenth of the rate: 279 us where this took 140 for 2048^3).
-// What rounds to infinity, infinities and NaN: the difference times zero is NaN there, and those four values are done again.
-__device__ __forceinline__ void split_tf32_special(uint32_t v, uint32_t& h, uint32_t& l) {
+// v = l / kLowScale - n + a rest below 2^-22 |v|: the high part negated, so that the subtraction needs no negation (both operands' are: h h' has its sign, and the
+// small products, negative, are subtracted); by integer rounding (the conversion instruction runs at a sixteenth of the rate: 279 us where this took 140 for
+// 2048^3).
+// The low part is held kLowScale times as large, so that it is not lost below the smallest normal value: unscaled, values of 2^-118 had 2^-20 of error and
+// those of 2^-125 kept eleven bits.  (With 2^12 the low part of what is cut off below would overflow.)  Of the bits behind its eleven the tensor core
+// takes no notice.
+// What rounds to infinity, infinities and NaN: the sum of the differences is not finite there, and those four values are done again.
+constexpr float kLowScale = 2048.f;
+__device__ __forceinline__ void split_tf32_special(uint32_t v, uint32_t& n, uint32_t& l) {
     const uint32_t a = v & 0x7fffffffu;
     if (a < 0x7f7ff000u) return;
-    h = a > 0x7f800000u ? 0x7fffffffu : v & 0xffffe000u;  // NaN; infinity, or cut off instead of rounded
-    l = a >= 0x7f800000u ? 0u : __float_as_uint(__uint_as_float(v) - __uint_as_float(h)) & 0xffffe000u;
+    n = a > 0x7f800000u ? 0x7fffffffu : (v & 0xffffe000u) ^ 0x80000000u;  // NaN; infinity, or cut off instead of rounded
+    l = a >= 0x7f800000u ? 0u : __float_as_uint((__uint_as_float(v) + __uint_as_float(n)) * kLowScale);
 }
-__device__ __forceinline__ void split_tf32(const uint4& v, uint32_t* h, uint32_t* l) {
+__device__ __forceinline__ void split_tf32(const uint4& v, uint32_t* n, uint32_t* l) {
     const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-    f32x2 z = 0ull;
+    f32x2 d[2];
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
-        h[j] = (in[j] + 0x1000u) & 0xffffe000u;
-        h[j + 1] = (in[j + 1] + 0x1000u) & 0xffffe000u;
-        const f32x2 d = add2(make_x2(__uint_as_float(in[j]), __uint_as_float(in[j + 1])), make_x2(-__uint_as_float(h[j]), -__uint_as_float(h[j + 1])));
-        z = fma2(d, 0ull, z);
-        const float2 f = split_x2(d);
-        l[j] = (__float_as_uint(f.x) + 0x1000u) & 0xffffe000u;
-        l[j + 1] = (__float_as_uint(f.y) + 0x1000u) & 0xffffe000u;
+        n[j] = ((in[j] + 0x1000u) & 0xffffe000u) ^ 0x80000000u;
+        n[j + 1] = ((in[j + 1] + 0x1000u) & 0xffffe000u) ^ 0x80000000u;
+        d[j / 2] = add2(make_x2(__uint_as_float(in[j]), __uint_as_float(in[j + 1])), make_x2(__uint_as_float(n[j]), __uint_as_float(n[j + 1])));
+        const float2 f = split_x2(mul2(d[j / 2], both(kLowScale)));
+        l[j] = __float_as_uint(f.x) + 0x1000u;
+        l[j + 1] = __float_as_uint(f.y) + 0x1000u;
     }
-    const float2 zf = split_x2(z);
-    if (!(zf.x + zf.y == 0.f)) {
+    const float2 z = split_x2(add2(d[0], d[1]));
+    if (!(fabsf(z.x + z.y) < INFINITY)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_tf32_special(in[j], h[j], l[j]);
+        for (int j = 0; j < 4; ++j) split_tf32_special(in[j], n[j], l[j]);
     }
 }
 
@@ -381,8 +387,9 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
         const uint32_t column0 = (uint32_t)(part * kCols), lanes = tmem + ((uint32_t)quarter << 16) + column0;
         float acc[kCols] = {};
         got = true;
-        // Adds columns of TMEM; `finite`: only to sums that are -- next to an infinity the small products are NaN (infinity times l = 0).
-        auto add = [&](uint32_t at, bool finite) {
+        // Adds columns of TMEM: a chain's, or subtracts the small products', which are kLowScale times as large -- these only from sums that are finite: next to an
+        // infinity they are NaN (infinity times l = 0).
+        auto add = [&](uint32_t at, bool small) {
 #pragma unroll
             for (int c = 0; c < kCols / 16; ++c) {
                 uint32_t r[16];
@@ -390,7 +397,7 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
                 tmem_ld_wait16(r);
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    if (!finite || fabsf(acc[c * 16 + j]) < INFINITY) acc[c * 16 + j] += __uint_as_float(r[j]);
+                    if (!small || fabsf(acc[c * 16 + j]) < INFINITY) acc[c * 16 + j] += __uint_as_float(r[j]) * (small ? -1.f / kLowScale : 1.f);
             }
         };
         // The accumulators start from zeros that are written: an instruction adds to those of a chain and of the small products together.
