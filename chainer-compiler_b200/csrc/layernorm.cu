@@ -419,14 +419,16 @@ __global__ void __launch_bounds__(512) layernorm_grad_kernel(const T* __restrict
 // and hide each other's latencies; the second pass reads shared memory again instead of holding both rows.  The columns' sums stay in registers.
 // Rows too long for the registers of 512 threads: the CL blocks of a cluster take a share of the columns each (one group per block), and the rows'
 // sums meet across them; one block with its sums in shared memory took 153 us for [4096, 16384] bf16 and 280 for [4096, 12345].
-// (A wait that expires raises the status word; the loop then runs on to its end over whatever is there, so that no barrier is missed.)
+// (A wait that expires raises the status word; the loop then runs on to its end over whatever is there, so that no barrier is missed.
+// test_skip: the row of a group whose copies are left out, chxq_tc_test_hooks.)
 // [8192, 8192] bf16: 86 us, 73% of a copy's rate (the instructions of two passes over 16-bit values bound it); [16384, 4096] fp32 122 us, the
 // memory's; [8192, 8192] fp32 140 us (89%); [4096, 16384] bf16 102 us, [4096, 12345] bf16 103 us, [4096, 14001] fp32 137 us.
 constexpr int kMaxStages = 8;
 template <typename T, int NV, bool SHIFT, int CL, int ROWS>
 __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, FloatArray scale,
                                                                   const float* __restrict__ mean, const float* __restrict__ inv, int64_t rows, int D, int G, int stages,
-                                                                  int row_bytes, T* __restrict__ dx, float* __restrict__ part, int* status, uint64_t wait_limit_ns) {
+                                                                  int row_bytes, T* __restrict__ dx, float* __restrict__ part, int* status, uint64_t wait_limit_ns,
+                                                                  int test_skip) {
     // (row_bytes: of a block's share of a row)
     constexpr int VEC = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) uint8_t ring[];  // [groups][stages][x, dy][row_bytes]; the block's sums [2][D] in the end
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
             }
         }
         tc::mbar_expect_tx(bar(stage), 2u * (uint32_t)bytes);
-        if (bytes > 0) {
+        if (bytes > 0 && k != test_skip) {
             bulk_load(tc::smem_u32(st), x + r * ldx + start, (uint32_t)bytes, bar(stage));
             bulk_load(tc::smem_u32(st + row_bytes), dy + r * lddy + start, (uint32_t)bytes, bar(stage));
         }
@@ -552,8 +554,9 @@ __global__ void __launch_bounds__(512) layernorm_grad_ring_kernel(const T* __res
             __syncwarp();
             tc::cluster_sync_all();
         }
-        // every thread has left the rows before these: theirs are the stages to refill
-        if (at.t == 0 && k >= ROWS)
+        // every thread has left the rows before these: theirs are the stages to refill (but none behind an expired wait: its barrier is still in the phase that
+        // a refill has arrived at)
+        if (at.t == 0 && k >= ROWS && !*static_cast<volatile int*>(&abort_flag))
 #pragma unroll
             for (int u = 0; u < ROWS; ++u)
                 if (k - ROWS + u + stages < n) fetch(k - ROWS + u + stages, old[u]);
@@ -855,7 +858,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
                     auto go = [&](auto* kernel) {
                         CHXQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, room));
                         CHXQ_CUDA(launch_pdl_cluster(cl, kernel, dim3((unsigned)(p.blocks * cl)), p.G * p.groups, smem, s, g, lddy, v, ldx, sc, mean, inv_std_dev, rows, (int)D,
-                                                     p.G, stages, row_bytes, static_cast<T*>(dx), part, status, (uint64_t)tc::wait_limit_ns_value()));
+                                                     p.G, stages, row_bytes, static_cast<T*>(dx), part, status, (uint64_t)tc::wait_limit_ns_value(), tc::test_skip_kb_value()));
                         count_launch(1);
                         return CHXQ_OK;
                     };

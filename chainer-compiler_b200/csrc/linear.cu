@@ -399,5 +399,6 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     a.status = device_status_ptr();
     if (!a.status) return set_error(CHXQ_ERR_CUDA, "device status word is unavailable");
     a.wait_limit_ns = (unsigned long long)tc::wait_limit_ns_value();
+    a.test_skip_kb = tc::test_skip_kb_value();
     return with_float_type(p->dtype, [&](auto t) { return launch_tc<decltype(t)>(*p, op, a, s); });
 }

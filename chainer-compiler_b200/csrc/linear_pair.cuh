@@ -112,7 +112,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     if (is_x) {
                         if (rank == 0) mbar_expect_tx(full(stage), 2 * Cfg::kStage);
                         tma_load_2d_pair(dst, &tmX, fb, kb * 128, row);
-                    } else {
+                    } else if (kb != p.test_skip_kb) {
                         tma_load_2d_pair(dst + Cfg::kTile, &tmW, fb, kb * 128, row);
                     }
                     if (++stage == kStages) {

@@ -19,6 +19,7 @@ struct TcArgs {
     int vec;  // rows of y and of the residual start on 16-byte boundaries and hold whole groups of 16 bytes
     int* status;
     unsigned long long wait_limit_ns;
+    int test_skip_kb;  // K block whose rows of w are not loaded (chxq_tc_test_hooks)
 };
 
 // Instruction descriptor of tcgen05.mma kind::f16: 32-bit accumulator, both operands K-major and of one type.

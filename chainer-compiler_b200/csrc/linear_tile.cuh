@@ -168,8 +168,9 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(const __grid_constant_
             if (!mbar_wait(empty(s), ((uint32_t)((kb - kb0) / STAGES) & 1u) ^ 1u, abort_flag, p.status, 41, 0, p.wait_limit_ns)) break;
             uint8_t* st = smem + s * Cfg::kStage;
             mbar_expect_tx(full(s), is_w ? Cfg::kTileW : Cfg::kTileX);
-            if (is_w) tma_load_2d(smem_u32(st), &tmW, full(s), kb * 128, w0);
-            else tma_load_2d(smem_u32(st + Cfg::kTileW), &tmX, full(s), kb * 128, x0);
+            if (is_w) {
+                if (kb != p.test_skip_kb) tma_load_2d(smem_u32(st), &tmW, full(s), kb * 128, w0);
+            } else tma_load_2d(smem_u32(st + Cfg::kTileW), &tmX, full(s), kb * 128, x0);
         }
     } else if (lane == 0 && warp == 1) {
         bool ok = true;
@@ -349,8 +350,9 @@ __global__ void __launch_bounds__(640) linear_tile_f32_kernel(const __grid_const
                 if (!mbar_wait(empty(s), ((uint32_t)(kb / STAGES) & 1u) ^ 1u, abort_flag, p.status, 61, 0, p.wait_limit_ns)) break;
                 uint8_t* st = smem + s * Cfg::kStage;
                 mbar_expect_tx(full(s), is_w ? Cfg::kTileW : Cfg::kTileX);
-                if (is_w) tma_load_2d(smem_u32(st), &tmW, full(s), (kb0 + kb) * 128, w0);
-                else tma_load_2d(smem_u32(st + x_high(kb)), &tmX, full(s), (kb0 + kb) * 128, x0);
+                if (is_w) {
+                    if (kb0 + kb != p.test_skip_kb) tma_load_2d(smem_u32(st), &tmW, full(s), (kb0 + kb) * 128, w0);
+                } else tma_load_2d(smem_u32(st + x_high(kb)), &tmX, full(s), (kb0 + kb) * 128, x0);
             }
         } else if (lane == 0 && warp == 1) {
             bool ok = true;

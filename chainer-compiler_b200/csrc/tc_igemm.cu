@@ -98,6 +98,9 @@ namespace tc {
 long long wait_limit_ns_value() {
     return g_wait_limit_ns.load(std::memory_order_relaxed);
 }
+int test_skip_kb_value() {
+    return g_test_skip_kb.load(std::memory_order_relaxed);
+}
 
 int encode_nhwc_box_map(CUtensorMap* out, const void* base, int C, int W, int H, int N, int64_t cs, int box_c, int box_w, int box_h) {
     EncodeTiledFn encode = get_encode_fn();
@@ -648,8 +651,8 @@ extern "C" int chxq_tl_read(long long* host) {
 }
 #endif
 
-// Test hooks of the bounded device-side waits (one-tile kernel): the time without progress after which a wait gives up, and the
-// K block whose weight load the producer leaves out (-1: none), so that a test can make a wait run out without faulting anything.
+// Test hooks of the bounded device-side waits: the time without progress after which a wait gives up, and the K block whose weight load a
+// producer leaves out (-1: none), so that a test can make a wait run out without faulting anything.
 extern "C" int chxq_tc_test_hooks(int64_t wait_limit_ns, int32_t skip_weight_load_kb) {
     if (wait_limit_ns < 1000000 || wait_limit_ns > 10000000000ll)
         return chxq::set_error(CHXQ_ERR_INVALID_ARGUMENT, "chxq_tc_test_hooks: the wait limit must lie between 1 ms and 10 s");
