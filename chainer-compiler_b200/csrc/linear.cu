@@ -273,10 +273,13 @@ int launch_rows(const chxq_linear_params& q, const LinearEpilogue& e, cudaStream
 
 // Which products they take.  Up to eight rows of fp32, and more of any type in blocks of eight where those run in two waves (two are on an SM at once).
 // 16-bit tiles read the weights as fast and convert none: they are left what takes longer than the start of a tile, about 2 us + (0.32 + 0.047 M) us per
-// 2^20 weights here against 4.6 + 0.305.  Rows off 16-byte boundaries, read value by value here, tiles copy first.  In us here and in tiles: [1, 1024] x
-// [4096, 1024]^T bf16 3.8 and 6.2, [8, 1024] x [4096, 1024]^T 5.4 and 6.3, [8, 4096] x [4096, 4096]^T 13.4 and 8.3, [64, 2000] x [64, 2000]^T fp16 3.1 and
-// 6.8, [4, 1023] x [4096, 1023]^T fp16 9.1 and 11.2; fp32: [64, 8192] x [64, 8192]^T 5.4 and 27, [411, 2000] x [16, 2000]^T 5.4 and 11.8, [64, 2048] x [250,
-// 2048]^T 10.1 and 12.2.
+// 2^20 weights here against 4.6 + 0.305.  Rows off 16-byte boundaries, read value by value here, tiles copy first: up to four rows of x gain by that at all
+// sizes but those of many short rows, more of them as long as 2^22 weights for every eight rows are read.  In us here and in tiles, x and w off 16-byte
+// boundaries, bf16: [4, 2001] x [2048, 2001]^T 8.7 and 10.5, [4, 4001] x [4096, 4001]^T 25.7 and 21.6, [8, 1001] x [4096, 1001]^T 11.8 and 11.9, [8, 4001] x
+// [1000, 4001]^T 9.6 and 11.3, [8, 8001] x [1000, 8001]^T 16.9 and 15.9, [16, 1001] x [1000, 1001]^T 6.3 and 7.3, [16, 4001] x [1000, 4001]^T 17.3 and 11.4,
+// [64, 8001] x [64, 8001]^T 9.0 and 11.8, [64, 8001] x [256, 8001]^T 34.4 and 13.3.  On them: [1, 1024] x [4096, 1024]^T bf16 3.8 and 6.2, [8, 1024] x [4096,
+// 1024]^T 5.4 and 6.3, [8, 4096] x [4096, 4096]^T 13.4 and 8.3, [64, 2000] x [64, 2000]^T fp16 3.1 and 6.8; fp32: [64, 8192] x [64, 8192]^T 5.4 and 27,
+// [411, 2000] x [16, 2000]^T 5.4 and 11.8, [64, 2048] x [250, 2048]^T 10.1 and 12.2.
 // And rows of more than 2^30 bytes, whatever their number: TMA counts a row's bytes in 32 signed bits.
 bool few_rows(const chxq_linear_params& q) {
     if (q.K * float_size(q.dtype) > kMostCoordinate) return true;
@@ -284,7 +287,7 @@ bool few_rows(const chxq_linear_params& q) {
     if (q.dtype == CHXQ_FLOAT32) return true;
     const int64_t values = q.O * q.K;
     if (rows16(q.x, q.ldx, q.M, 2) && rows16(q.w, q.ldw, q.O, 2)) return values * (1 + 3 * q.M) <= 110000000;
-    return q.M <= 4 || values <= 4200000;
+    return q.M <= 4 || values * ((q.M + 7) / 8) <= 1ll << 22;
 }
 
 }  // namespace

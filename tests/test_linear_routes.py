@@ -46,6 +46,16 @@ def test_rows_whose_bytes_pass_the_coordinates_of_tma(pkg, dtype, size):
         assert route(pkg, 1, 1 << 28, 8, dtype) == _lib.LINEAR_TILES
 
 
+def test_rows_off_16_byte_boundaries(pkg):
+    """Read value by value: as long as all blocks of eight rows of x together read no more than 2^22 weights, and always for four rows."""
+    from chainer_compiler_b200 import _lib
+    for dtype in ("float16", "bfloat16"):
+        for m, k, o in ((4, 8001, 4096), (8, 1001, 4096), (8, 4001, 1000), (16, 1001, 1000), (64, 8001, 64)):
+            assert route(pkg, m, k, o, dtype) == _lib.LINEAR_ROWS
+        for m, k, o in ((8, 8001, 1000), (16, 4001, 1000), (64, 8001, 256), (64, 2001, 1000)):
+            assert route(pkg, m, k, o, dtype) == _lib.LINEAR_TILES
+
+
 def test_refusals(pkg):
     from chainer_compiler_b200 import _lib
     bad = -_lib.ERR_INVALID_ARGUMENT
