@@ -49,8 +49,9 @@ __device__ __forceinline__ f32x2 both(float v) {
     return make_x2(v, v);
 }
 
-// Two values at a time for 16-bit outputs, with exponential and reciprocal by the approximate instructions: a few 2^-22 relative, a thousandth of the
-// output's rounding.
+// Two values at a time for 16-bit outputs, with exponential and reciprocal by the approximate instructions: a few 2^-22 relative near zero.  Further out the
+// exponent, which is rounded at its own size, adds 2^-24 of its magnitude (base 2): 18 x 2^-22 for Gelu at z = -10, 8 x 2^-22 for Swish at z = -80, still a
+// thousandth of bf16's rounding, and fp16 has no such values.  Exponentials and reciprocals below 2^-126 count as zero (Swish and Sigmoid below -87.3).
 // Gelu: erfc by the Chebyshev fit of Press et al., Numerical Recipes, 6.2 ("erfcc", fractional error below 1.2e-7 everywhere): for u >= 0
 // erfc(u) = t exp(P(t) - u^2), t = 1 / (1 + u / 2); here with P and u^2 times log2 e.  [4096, 1024] x [4096, 1024]^T with Gelu on one B200: 55 us with
 // CUDA's erfcf.

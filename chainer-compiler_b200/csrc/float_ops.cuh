@@ -106,9 +106,8 @@ struct Pack {
         }
     }
     __device__ __forceinline__ void store(T* p) const {
-        if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-        else *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+        static_assert(kBytes == 16, "a 16-byte access");
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -205,42 +204,19 @@ struct Pack {
             return *reinterpret_cast<const T*>(&h);
         }
     }
-    __device__ __forceinline__ void set(const float (&f)[N]) {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) w[i] = __float_as_uint(f[i]);
-        } else if constexpr (N == 1) {
-            const T h = from_f32<T>(f[0]);
-            w[0] = *reinterpret_cast<const uint16_t*>(&h);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[i], f[i + 1]);
-                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                } else {
-                    const __half2 h = __floats2half2_rn(f[i], f[i + 1]);
-                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
-        }
-    }
 };
 
-// N consecutive values of a parameter array (N from a Pack of some 2-, 4- or 16-byte access; the array starts on a 16-byte boundary where N > 1).
+// N consecutive values of a parameter array for a row's 16-byte piece: N = 8 beside a 16-bit type, or 4 beside float32, whose parameters are float32 too.  The
+// array starts on a 16-byte boundary.
 template <int N>
 __device__ __forceinline__ void load_params(const FloatArray& a, int64_t i, float (&f)[N]) {
-    if (a.dtype == CHXQ_FLOAT32) {
+    static_assert(N == 4 || N == 8, "a 16-byte piece");
+    if (N == 4 || a.dtype == CHXQ_FLOAT32) {
         const float* p = static_cast<const float*>(a.p) + i;
-        if constexpr (N >= 4) {
 #pragma unroll
-            for (int j = 0; j < N; j += 4) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(p + j));
-                f[j] = v.x; f[j + 1] = v.y; f[j + 2] = v.z; f[j + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) f[j] = __ldg(p + j);
+        for (int j = 0; j < N; j += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p + j));
+            f[j] = v.x; f[j + 1] = v.y; f[j + 2] = v.z; f[j + 3] = v.w;
         }
     } else if constexpr (N == 8) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.p) + i));
@@ -256,9 +232,6 @@ __device__ __forceinline__ void load_params(const FloatArray& a, int64_t i, floa
                 f[2 * j + 1] = h.y;
             }
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = load_param(a, i + j);
     }
 }
 

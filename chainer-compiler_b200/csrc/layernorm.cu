@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(BLOCK ? 1024 : 256) layernorm_kernel(const T* 
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j) a = add2(a, v[i][j]);
     }
-    const float rd = 1.f / (float)D;
+    const float rd = 1.f / (float)D;  // (its rounding, 2^-24, is far below that of a sum of D terms)
     float2 f = split_x2(a);
     const float m = sum(f.x + f.y, 0) * rd;
     a = 0ull;
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kThreads) layernorm_dparam_long_kernel(const T
 
 // part [shares][2 D] -> the sum of the shares: 32 columns a block; warps that take every eighth share (up to 40 shares) or every 32nd, at most five each,
 // loaded together.
-constexpr int kMaxBlocks = 148;  // of the gradient: one per SM
+constexpr int kMaxBlocks = 148;  // of the gradient, which the workspace has room for: one per SM of a B200
 __global__ void __launch_bounds__(1024) layernorm_join_kernel(const float* __restrict__ part, int shares, int64_t D, int dtype, void* dscale, void* dbias) {
     __shared__ float acc[32][33];
     pdl_launch_dependents();
@@ -711,10 +711,10 @@ struct Plan {
     int G, groups, blocks;
 };
 
-// Groups for `pieces` pieces of a row, nv each to a thread, in blocks of about `threads` threads, `per_sm` of them on an SM.  G is a power of two
+// Groups for `pieces` pieces of a row, nv each to a thread, in blocks of about `threads` threads, one on an SM.  G is a power of two
 // within a warp, and whole warps above.  Where a row starts at another place of a 16-byte piece than the one before (shift), the number of
 // blocks is a multiple of vec.
-Plan plan_rows(int64_t pieces, int nv, int64_t rows, int threads, int per_sm, bool shift, int vec) {
+Plan plan_rows(int64_t pieces, int nv, int64_t rows, int threads, bool shift, int vec) {
     Plan p;
     const int64_t t = (pieces + nv - 1) / nv;
     p.G = 1;
@@ -722,8 +722,9 @@ Plan plan_rows(int64_t pieces, int nv, int64_t rows, int threads, int per_sm, bo
     if (t > 32) p.G = (int)((t + 31) / 32 * 32);
     const int least = std::max(1, 32 / p.G);  // whole warps
     p.groups = std::max(least, threads / p.G);
-    while (p.groups > least && (int64_t)p.groups * 148 > 2 * rows) p.groups = std::max(least, p.groups / 2);  // few rows: on more SMs
-    int64_t blocks = std::min<int64_t>((rows + p.groups - 1) / p.groups, (int64_t)148 * per_sm);
+    const int64_t sms = std::min(tc::sm_count(), kMaxBlocks);
+    while (p.groups > least && p.groups * sms > 2 * rows) p.groups = std::max(least, p.groups / 2);  // few rows: on more SMs
+    int64_t blocks = std::min<int64_t>((rows + p.groups - 1) / p.groups, sms);
     if (shift) blocks = blocks > vec ? blocks / vec * vec : vec;  // not more than fit the SMs at a time
     p.blocks = (int)blocks;
     return p;
@@ -798,7 +799,7 @@ extern "C" int chxq_layernorm(const void* x, int64_t ldx, int32_t dtype, const v
                 return pieces == 4 * threads ? go(layernorm_kernel<T, 4, true, false, true>) : go(layernorm_kernel<T, 4, true, false, false>);
             }
         }
-        layernorm_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kThreads, 0, s>>>(static_cast<const T*>(x), ldx, g, b, rows, D, epsilon,
+        layernorm_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, tc::sm_count() * 8), kThreads, 0, s>>>(static_cast<const T*>(x), ldx, g, b, rows, D, epsilon,
                                                                                                  static_cast<T*>(y), mean, inv_std_dev);
         CHXQ_LAUNCH_CHECK();
         return CHXQ_OK;
@@ -840,7 +841,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
             const int nv = VEC == 4 && pieces > 1024 ? 4 : 2, cl = pieces <= nv * 512 ? 1 : (pieces <= nv * 1024 ? 2 : 4);
             if (same_places(bits, rows, ldx, D, VEC) && same_places(bits, rows, lddy, D, VEC) && pieces <= (VEC == 4 ? 4 : 2) * (VEC == 4 ? 1024 : 2048)) {
                 const int64_t share = (pieces + cl - 1) / cl;
-                Plan p = plan_rows(share, nv, rows, 512, 1, shift, VEC);
+                Plan p = plan_rows(share, nv, rows, 512, shift, VEC);
                 if (cl > 1) {
                     const int64_t most = cl == 2 ? 74 : 32;  // clusters that are resident at once (of four: 33)
                     p.blocks = (int)std::min<int64_t>(std::max<int64_t>(rows, 1), most);
@@ -881,7 +882,7 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
                 };
                 return shift ? go(layernorm_grad_kernel<T, 2, true>) : go(layernorm_grad_kernel<T, 2, false>);
             }
-            layernorm_dx_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kThreads, 0, s>>>(g, lddy, v, ldx, sc, mean, inv_std_dev, rows, D, static_cast<T*>(dx));
+            layernorm_dx_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, tc::sm_count() * 8), kThreads, 0, s>>>(g, lddy, v, ldx, sc, mean, inv_std_dev, rows, D, static_cast<T*>(dx));
             CHXQ_LAUNCH_CHECK();
             shares = (int)std::min<int64_t>(rows, grad_shares(D));
             layernorm_dparam_long_kernel<T><<<dim3((unsigned)((D + kThreads - 1) / kThreads), shares), kThreads, 0, s>>>(g, lddy, v, ldx, mean, inv_std_dev, rows, D, part);

@@ -97,7 +97,7 @@ int cluster_slots(F* kernel, int cluster, int threads, int smem, KernelState& st
     int n = st.slots[dev][cluster].load(std::memory_order_acquire);
     if (n > 0) return n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cluster * 148));
+    cfg.gridDim = dim3((unsigned)(cluster * tc::sm_count()));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cudaLaunchAttribute at[1];
@@ -358,7 +358,7 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
     cudaStream_t s = as_stream(stream);
     if (p->K == 0)
         return with_float_type(p->dtype, [&](auto t) {
-            linear_empty_kernel<decltype(t)><<<(unsigned)std::min<int64_t>((p->M * p->O + 255) / 256, 148 * 8), 256, 0, s>>>(p->M, p->O, e);
+            linear_empty_kernel<decltype(t)><<<(unsigned)std::min<int64_t>((p->M * p->O + 255) / 256, tc::sm_count() * 8), 256, 0, s>>>(p->M, p->O, e);
             CHXQ_LAUNCH_CHECK();
             return CHXQ_OK;
         });
@@ -388,7 +388,7 @@ extern "C" int chxq_linear(const chxq_linear_params* p, void* workspace, size_t 
             op.ldw = pitch;
         }
         const int64_t blocks = ((jx.rows + jw.rows) * (pitch * size / 16) + 255) / 256;
-        CHXQ_CUDA(launch_pdl(size == 4 ? align_rows_kernel<uint32_t> : align_rows_kernel<uint16_t>, dim3((unsigned)std::min<int64_t>(blocks, 148 * 16)), 256, 0, s, jx, jw,
+        CHXQ_CUDA(launch_pdl(size == 4 ? align_rows_kernel<uint32_t> : align_rows_kernel<uint16_t>, dim3((unsigned)std::min<int64_t>(blocks, tc::sm_count() * 16)), 256, 0, s, jx, jw,
                              p->K, pitch));
         count_launch(1);
     }

@@ -171,7 +171,6 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             int mb, ob;
             coords(item, mb, ob);
             const int m0 = mb * 256 + (int)rank * 128, o0 = ob * 256;
-            const int64_t m = m0 + row;
             if (a.tma_res && issuer) {
                 fetch_residual(o0 + group * 64, m0);
                 if (o0 + (group + 2) * 64 < p.O)

@@ -143,7 +143,6 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
     const int p0 = (int)((int64_t)pieces * rank / split), p1 = (int)((int64_t)pieces * (rank + 1) / split);
     const T* body = x + head;
     constexpr int kLanes = W * 32;
-    const int t = W == 1 ? lane : (int)threadIdx.x;
 
     float m = -INFINITY;
     f32x2 s2 = 0ull, t2 = 0ull;
@@ -461,9 +460,10 @@ extern "C" int chxq_token_logprobs(const void* logits, int64_t ld, int32_t dtype
         // A warp per row where there are rows enough for half of the warps that fit; else a block, or a cluster of them as long as the blocks
         // do not fill the SMs twice and each still has a round of its accesses.
         const int round = kThreads * 4 * 16 / (int)sizeof(T);
+        const int64_t sms = tc::sm_count();
         int split = 1;
-        while (split < 8 && rows * split < 2 * 148 && V >= (int64_t)round * split * 2) split *= 2;
-        const bool warps = V <= 16384 && rows >= 148 * 8;
+        while (split < 8 && rows * split < 2 * sms && V >= (int64_t)round * split * 2) split *= 2;
+        const bool warps = V <= 16384 && rows >= sms * 8;
         const int64_t grid = warps ? (rows + kWarps - 1) / kWarps : rows * split;
         if (grid >= (1ll << 31)) return set_error(CHXQ_ERR_UNSUPPORTED, "TokenLogProbs: too many rows");
         auto go = [&](auto* kernel) {

@@ -9,6 +9,7 @@
 #include "kernels.h"
 #include "linear_chain.cuh"
 #include "pdl.cuh"
+#include "tc_launch.h"
 
 namespace chxq {
 namespace {
@@ -897,7 +898,8 @@ extern "C" int chxq_global_avgpool_dq_nhwc(const uint8_t* x, int32_t N, int32_t 
 // [1024, 1000] x [1000, 1000]^T 76, 73, 115; [512, 19] x [1500, 19]^T 5.6, 6.9, 11.0; [30, 333] x [10000, 333]^T 19.9, 45, 42.
 static void launch_linear_large(const float* x, const float* w, const float* b, int N, int K, int O, float* y, bool rows16, cudaStream_t s) {
     auto blocks = [&](int bm, int bn) { return (int64_t)((N + bm - 1) / bm) * ((O + bn - 1) / bn); };
-    auto cost = [&](int bm, int bn, double one, double more) { return (blocks(bm, bn) + 147) / 148 * bm * bn * (blocks(bm, bn) > 148 ? more : one); };
+    const int sms = tc::sm_count();
+    auto cost = [&](int bm, int bn, double one, double more) { return (blocks(bm, bn) + sms - 1) / sms * bm * bn * (blocks(bm, bn) > sms ? more : one); };
     const double small = cost(32, 64, 19.5, 19.5), wide = cost(128, 64, 17, 13.5), large = cost(128, 128, 17, 12);
     if (small <= wide && small <= large) {
         linear_f32_regs_kernel<<<dim3((O + 63) / 64, (N + 31) / 32), kLinThreads, 0, s>>>(x, w, b, N, K, O, y);

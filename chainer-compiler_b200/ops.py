@@ -279,7 +279,8 @@ def Linear(x, w, b=None, activation=None, residual=None, residual_first=False):
 
     x [..., K] and w [O, K] are float32, float16 or bfloat16; b [O] has their type or float32; residual has y's shape and type.
     activation: None, "Relu", "Gelu" (erf), "GeluTanh", "Swish" (z * sigmoid(z)), "Sigmoid" or "Tanh".  Sums are held in 32 bits and rounded
-    once, after the epilogue.  Rows of x, w and residual may be cut out of wider ones (x[:, :K]); other strides are copied.
+    once, after the epilogue; 16-bit products on tensor cores cut them off between steps, by at most K 2^-27 of a sum of terms of one sign.
+    Rows of x, w and residual may be cut out of wider ones (x[:, :K]); other strides are copied.
     float32 without activation and residual keeps one k-ascending chain of fused multiply-adds per output, whatever the sizes.  float32 with
     either, for more than a few rows, runs on tensor cores that take 22 bits of each operand (2^-21 of every product; subnormal values to a unit
     or two of 2^-149), the sums in 32 bits."""

@@ -390,6 +390,7 @@ int chxq_conv_integer_dev_ws(const void* x, const void* w, const chxq_conv_geom*
  *   y[m, o] = act(sum_k x[m, k] w[o, k] + bias[o]) + residual[m, o], or, with residual_first, act(... + residual[m, o]).
  * x [M, ldx], w [O, ldw], residual [M, ldr] and y [M, ldy] have the type `dtype`; bias [O] has it too or is fp32; bias and residual may be
  * NULL.  y may be the residual's memory (same ldy and ldr), and none of the other operands'.
+ * 16-bit products for more than a few rows cut their sums off between steps, by at most K 2^-27 of a sum of terms of one sign.
  * CHXQ_FLOAT32 for more than a few rows: 22 bits of each operand (2^-21 of every product; subnormal values to a unit or two of 2^-149).
  * chxq_linear_workspace reads the extents, pitches and the alignment of the addresses. */
 typedef struct chxq_linear_params {
