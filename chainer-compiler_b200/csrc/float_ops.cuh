@@ -20,6 +20,12 @@ inline int float_size(int dtype) {
     return dtype == CHXQ_FLOAT32 ? 4 : 2;
 }
 
+// Whether addresses are multiples of the size of the values there: an access elsewhere faults.
+template <typename... P>
+inline bool on_values_of(int size, const P*... p) {
+    return (((uintptr_t)0 | ... | reinterpret_cast<uintptr_t>(p)) & (uintptr_t)(size - 1)) == 0;
+}
+
 __device__ __forceinline__ float to_f32(float v) {
     return v;
 }

@@ -768,6 +768,8 @@ extern "C" int chxq_layernorm(const void* x, int64_t ldx, int32_t dtype, const v
     if (rc != CHXQ_OK) return rc;
     if (rows == 0) return CHXQ_OK;
     CHXQ_CHECK_ARG(x && scale && y && (rows == 1 || ldx >= D), "LayerNormalization: bad arguments");
+    CHXQ_CHECK_ARG(on_values_of(float_size(dtype), x, y) && on_values_of(float_size(affine_dtype), scale, bias) && on_values_of(4, mean, inv_std_dev),
+                   "LayerNormalization: an address is no multiple of its values' size");
     cudaStream_t s = as_stream(stream);
     const FloatArray g = {scale, affine_dtype}, b = {bias, affine_dtype};
     return with_float_type(dtype, [&](auto t) {
@@ -822,6 +824,9 @@ extern "C" int chxq_layernorm_grad(const void* dy, int64_t lddy, const void* x, 
     const int rc = check_norm("LayerNormalizationGrad", dtype, affine_dtype, rows, D);
     if (rc != CHXQ_OK) return rc;
     CHXQ_CHECK_ARG(dscale && scale && (rows == 0 || (dy && x && mean && inv_std_dev && dx)) && (rows <= 1 || (ldx >= D && lddy >= D)), "LayerNormalizationGrad: bad arguments");
+    CHXQ_CHECK_ARG(on_values_of(float_size(dtype), dy, x, dx) && on_values_of(float_size(affine_dtype), scale, dscale, dbias) &&
+                           on_values_of(4, mean, inv_std_dev, workspace),
+                   "LayerNormalizationGrad: an address is no multiple of its values' size");
     const size_t need = chxq_layernorm_grad_workspace(rows, D);
     if (!workspace || workspace_bytes < need) return set_error(CHXQ_ERR_WORKSPACE, "LayerNormalizationGrad: needs %zu bytes of workspace", need);
     float* part = static_cast<float*>(workspace);

@@ -305,6 +305,8 @@ static int check_linear(const chxq_linear_params* p) {
                            (!p->residual || p->M == 1 || p->ldr >= p->O),
                    "Linear: rows overlap");
     CHXQ_CHECK_ARG(!p->bias || p->bias_dtype == p->dtype || p->bias_dtype == CHXQ_FLOAT32, "Linear: the bias must be float32 or have the operands' type");
+    CHXQ_CHECK_ARG(on_values_of(float_size(p->dtype), p->x, p->w, p->residual, p->y) && (!p->bias || on_values_of(float_size(p->bias_dtype), p->bias)),
+                   "Linear: an address is no multiple of its values' size");
     CHXQ_CHECK_ARG(p->activation >= CHXQ_ACT_NONE && p->activation <= CHXQ_ACT_TANH, "Linear: unknown activation %d", p->activation);
     return CHXQ_OK;
 }

@@ -453,6 +453,9 @@ extern "C" int chxq_token_logprobs(const void* logits, int64_t ld, int32_t dtype
     CHXQ_CHECK_ARG(num_top >= 0 && num_top <= CHXQ_MAX_TOP && num_top <= V, "TokenLogProbs: num_top must be at most %d and at most the number of logits", CHXQ_MAX_TOP);
     if (rows == 0) return CHXQ_OK;
     CHXQ_CHECK_ARG(logits && tokens && logprob && entropy && log_sum_exp && (num_top == 0 || (top_logprobs && top_tokens)), "TokenLogProbs: null argument");
+    CHXQ_CHECK_ARG(on_values_of(float_size(dtype), logits) && on_values_of(token_dtype == CHXQ_INT64 ? 8 : 4, tokens) &&
+                           on_values_of(4, logprob, entropy, log_sum_exp, top_logprobs) && on_values_of(8, top_tokens),
+                   "TokenLogProbs: an address is no multiple of its values' size");
     const LogprobArgs a = {tokens, token_dtype, num_top, has_ignore, rows, ignore_index, logprob, entropy, log_sum_exp, top_logprobs, top_tokens};
     cudaStream_t s = as_stream(stream);
     return with_float_type(dtype, [&](auto t) {
@@ -483,6 +486,9 @@ extern "C" int chxq_token_logprobs_grad(const float* dlogprob, const float* dent
     if (rc != CHXQ_OK) return rc;
     if (rows == 0) return CHXQ_OK;
     CHXQ_CHECK_ARG(logits && tokens && log_sum_exp && dlogits && (!dentropy || entropy), "TokenLogProbsGrad: null argument");
+    CHXQ_CHECK_ARG(on_values_of(float_size(dtype), logits, dlogits) && on_values_of(token_dtype == CHXQ_INT64 ? 8 : 4, tokens) &&
+                           on_values_of(4, dlogprob, dentropy, log_sum_exp, entropy),
+                   "TokenLogProbsGrad: an address is no multiple of its values' size");
     cudaStream_t s = as_stream(stream);
     return with_float_type(dtype, [&](auto t) {
         using T = decltype(t);

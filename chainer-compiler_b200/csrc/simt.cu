@@ -915,6 +915,8 @@ static void launch_linear_large(const float* x, const float* w, const float* b, 
 extern "C" int chxq_linear_f32(const float* x, const float* w, const float* b, int32_t N, int32_t K, int32_t O, float* y, void* stream) {
     CHXQ_CHECK_ARG(x && w && y && N > 0 && K > 0 && O > 0, "Linear: bad arguments");
     CHXQ_CHECK_ARG(K <= INT32_MAX - 1024, "Linear: K = %d is too long for a float32 product without an epilogue", K);  // (slices of up to 128 are counted in 32 bits)
+    CHXQ_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(y)) & 3u) == 0,
+                   "Linear: an address is no multiple of its values' size");
     constexpr int kMostRows = 65535 * 32;  // of one launch
     for (; N > kMostRows; N -= kMostRows, x += (int64_t)kMostRows * K, y += (int64_t)kMostRows * O) {
         const int rc = chxq_linear_f32(x, w, b, kMostRows, K, O, y, stream);
