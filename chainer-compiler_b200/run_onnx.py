@@ -362,7 +362,8 @@ def fuse_linear(program, epilogue=True):
     """A float product with constant weights becomes one Linear instruction: MatMul [..., K] x [K, O], and Gemm without transA,
     alpha and beta (a float32 Gemm with transB is left as it is: the executor runs it as Linear already).  With `epilogue` it
     takes what follows it as single-use values: an Add of a constant [O] or [1, O] (the bias), then Relu, Tanh, Sigmoid, Gelu or x *
-    Sigmoid(x) and an Add of a computed value (the residual), in either order.  The weights are laid out as [O, K] once, here.
+    Sigmoid(x) and an Add of a computed value (the residual), in either order.  The weights are laid out as [O, K] once, here.  (float32
+    with an activation or a residual holds 22 bits of each operand for more than a few rows, as ops.Linear says.)
     Inputs: x, weights, bias or "", residual or "".  The replaced nodes stay in `members`, for the export."""
     insts = program.insts
     users = {}
